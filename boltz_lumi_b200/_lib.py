@@ -58,8 +58,16 @@ SIGNATURES = {
     "bl_layernorm_split3": [_p, c_int64, c_int64, _p, _p, c_float, _p, _p],
     "bl_adaln_modulate_split3": [_p, _p, _p, _p, c_int64, c_int64, c_float, _p],
     "bl_diffusion_epilogue_split3": [_p, _p, _p, _p, c_int64, c_int64, c_int, _p],
+    "bl_relative_position_encoding": [_p] * 6 + [c_int64] * 5 + [c_int, _p, c_int, c_int, _p],
+    "bl_relative_position_encoding_workspace": [c_int64] * 5,
+    "bl_relative_position_encoding_backward": [_p, c_int] + [_p] * 5 + [c_int64] * 5 + [c_int, _p, _p, c_int64, _p],
+    "bl_relative_position_bias": [_p] * 4 + [c_int64, _p, _p] + [c_int64] * 5 + [_p, c_int] + [c_int64] * 3 + [_p],
+    "bl_relative_position_bias_workspace": [c_int64] * 5,
+    "bl_relative_position_bias_backward": [_p, c_int] + [c_int64] * 3 + [_p] * 3 + [c_int64, _p, _p] + [c_int64] * 5
+                                          + [_p, _p, c_int64, _p],
 }
-_RESTYPES = {"bl_last_error": ctypes.c_char_p}
+_RESTYPES = {"bl_last_error": ctypes.c_char_p, "bl_relative_position_encoding_workspace": c_int64,
+             "bl_relative_position_bias_workspace": c_int64}
 
 _lib = None
 
@@ -152,6 +160,21 @@ def current_stream_handle() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def launch(device, name, *args):
+    """:func:`call` ``name(*args, stream)`` on torch's current stream of ``device``, whichever device is current."""
+    index = device.index
+    current = torch.cuda.current_device()
+    if index is None or index == current:
+        return call(name, *args, _raw_stream(current) if _raw_stream is not None else current_stream_handle())
+    with torch.cuda.device(device):
+        return call(name, *args, current_stream_handle())
+
+
+def size_of(name, *args):
+    """The value of a size query of the library (no status, no launch)."""
+    return getattr(load(), name)(*args)
 
 
 def ptr(tensor):

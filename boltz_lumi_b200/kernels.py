@@ -8,11 +8,12 @@ no fallback path.
 """
 
 import functools
+import math
 
 import torch
 
 from . import _lib
-from ._lib import call, ptr, stream_of
+from ._lib import call, launch, ptr, size_of, stream_of
 
 
 def _require_inference(*tensors):
@@ -382,3 +383,198 @@ def epilogue_split3(a, b, c, kind):
     call("bl_diffusion_epilogue_split3", a.data_ptr(), ptr(b), ptr(c), out.data_ptr(), rows, cols, kind,
          _lib.current_stream_handle())
     return out
+
+
+# ---------------------------------------------------------------------------
+# Relative positions by buckets
+# ---------------------------------------------------------------------------
+def _workspace(nbytes, device):
+    return torch.empty(max(int(nbytes), 16), device=device, dtype=torch.uint8)
+
+
+def _indices(device, shape, **tensors):
+    """Integer index tensors as contiguous int64 of ``shape`` on ``device`` (None stays None)."""
+    out = []
+    for name, t in tensors.items():
+        if t is not None:
+            if t.device != device:
+                raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+            if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+                raise RuntimeError(f"{name} must hold integers, got {t.dtype}")
+            if tuple(t.shape) != tuple(shape):
+                raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+            if t.dtype != torch.int64 or not t.is_contiguous():
+                t = t.to(torch.int64).contiguous()
+        out.append(t)
+    return out
+
+
+def _float_dtype(dtype, what):
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{what} must be fp32 or bf16, got {dtype}")
+    return dtype
+
+
+def relative_position_columns(r_max=32, s_max=2):
+    """Columns of the relative position encoding's weight: residue offsets, token offsets, entity, chain copies."""
+    return 2 * (2 * r_max + 2) + 1 + 2 * s_max + 2
+
+
+def relative_position_encoding(weight, residue_index, asym_id, entity_id, token_index, sym_id, r_max=32, s_max=2,
+                               fix_sym_check=False, out_dtype=None, residual=None):
+    """Relative position encoding of token pairs, [B, N, N, C] (AF3 supplementary Algorithm 3).
+
+    ``weight`` is upstream ``RelativePositionEncoder.linear_layer.weight``, fp32
+    [C, 4 r_max + 2 s_max + 7], C a multiple of 4; the token features are
+    integers [B, N].  Pair (i, j) gets the sum of the weight columns of its
+    clipped residue offset, token offset and chain-copy offset, and of the
+    entity column if the entities agree (``fix_sym_check``: the chain-copy
+    offset counts within an entity instead of between chains).  The sum is
+    fp32, rounded once to ``out_dtype`` (default fp32).  With ``residual`` (a
+    contiguous fp32 [B, N, N, C]) it is added into that tensor, which is
+    returned.  For gradients see :func:`relative_position_encoding_backward`
+    and :mod:`boltz_lumi_b200.autograd`.
+    """
+    _require_inference(weight, residual)
+    _require_cuda(weight, residue_index, residual)
+    if residue_index.dim() != 2:
+        raise RuntimeError("token features must be [B, N]")
+    b, n = residue_index.shape
+    if weight.dtype != torch.float32 or weight.dim() != 2 or weight.shape[1] != relative_position_columns(r_max, s_max):
+        raise RuntimeError(f"weight must be fp32 [C, {relative_position_columns(r_max, s_max)}] for r_max {r_max}, "
+                           f"s_max {s_max}, got {weight.dtype} {list(weight.shape)}")
+    c = weight.shape[0]
+    features = _indices(weight.device, (b, n), residue_index=residue_index, asym_id=asym_id, entity_id=entity_id,
+                        token_index=token_index, sym_id=sym_id)
+    if residual is not None:
+        if residual.dtype != torch.float32 or not residual.is_contiguous() or tuple(residual.shape) != (b, n, n, c):
+            raise RuntimeError(f"residual must be a contiguous fp32 tensor [{b}, {n}, {n}, {c}]")
+        if out_dtype not in (None, torch.float32):
+            raise RuntimeError("an fp32 residual keeps its dtype")
+        out = residual
+    else:
+        out = torch.empty(b, n, n, c, device=weight.device, dtype=_float_dtype(out_dtype or torch.float32, "out_dtype"))
+    weight = weight.contiguous()
+    launch(weight.device, "bl_relative_position_encoding", weight.data_ptr(), *(t.data_ptr() for t in features), b, n, c,
+           r_max, s_max, int(fix_sym_check), out.data_ptr(), _lib.dtype_code(out.dtype), int(residual is not None))
+    return out
+
+
+def relative_position_encoding_backward(grad, residue_index, asym_id, entity_id, token_index, sym_id, r_max=32, s_max=2,
+                                        fix_sym_check=False):
+    """Gradient of :func:`relative_position_encoding` with respect to its weight: fp32 [C, columns] from the
+    gradient of the output, fp32 or bf16 [B, N, N, C].  Sums are fp32 in a fixed order."""
+    _require_inference(grad)
+    _require_cuda(grad, residue_index)
+    if grad.dim() != 4 or grad.shape[1] != grad.shape[2]:
+        raise RuntimeError("grad must be [B, N, N, C]")
+    _float_dtype(grad.dtype, "grad")
+    b, n, _, c = grad.shape
+    device = grad.device
+    features = _indices(device, (b, n), residue_index=residue_index, asym_id=asym_id, entity_id=entity_id,
+                        token_index=token_index, sym_id=sym_id)
+    grad = grad.contiguous()
+    if grad.data_ptr() % 4:
+        grad = grad.clone()
+    dweight = torch.empty(c, relative_position_columns(r_max, s_max), device=device, dtype=torch.float32)
+    nbytes = size_of("bl_relative_position_encoding_workspace", b, n, c, r_max, s_max)
+    work = _workspace(nbytes, device)
+    launch(device, "bl_relative_position_encoding_backward", grad.data_ptr(), _lib.dtype_code(grad.dtype),
+           *(t.data_ptr() for t in features), b, n, c, r_max, s_max, int(fix_sym_check), dweight.data_ptr(),
+           work.data_ptr(), nbytes)
+    return dweight
+
+
+def clipped_buckets(max_distance, device="cuda"):
+    """Bucket table of :func:`relative_position_bias` with one bucket per offset clipped to
+    [-max_distance, max_distance] (int32, 2 max_distance + 1 buckets)."""
+    return torch.arange(2 * max_distance + 1, dtype=torch.int32, device=device)
+
+
+def log_spaced_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
+    """Bucket table of :func:`relative_position_bias` with log-spaced far offsets (int32, 2 max_distance + 1).
+
+    Half of the buckets (of each sign, with ``bidirectional``) hold one offset each; the others grow
+    geometrically up to ``max_distance``.  Offset = query position - key position; with
+    ``bidirectional`` keys ahead of the query (negative offsets) take the upper half of the buckets,
+    without it they share the bucket of offset 0.
+    """
+    side = num_buckets // 2 if bidirectional else num_buckets
+    exact = side // 2
+    if exact < 1 or max_distance <= exact:
+        raise RuntimeError("log_spaced_buckets needs num_buckets >= 4 (2 one-sided) and a larger max_distance")
+    lut = []
+    for offset in range(-max_distance, max_distance + 1):
+        m = abs(offset) if bidirectional else max(offset, 0)
+        if m >= exact:
+            m = min(side - 1, exact + int(math.log(m / exact) / math.log(max_distance / exact) * (side - exact)))
+        lut.append(m + (side if bidirectional and offset < 0 else 0))
+    return torch.tensor(lut, dtype=torch.int32, device=device)
+
+
+def _bias_positions(device, q_pos, k_pos, lut, q_group, k_group):
+    if q_pos.dim() != 2 or k_pos.dim() != 2 or q_pos.shape[0] != k_pos.shape[0]:
+        raise RuntimeError("q_pos must be [B, Nq] and k_pos [B, Nk]")
+    if (q_group is None) != (k_group is None):
+        raise RuntimeError("give both q_group and k_group or neither")
+    if lut.dim() != 1 or lut.dtype != torch.int32 or lut.numel() % 2 == 0 or lut.device != device:
+        raise RuntimeError("lut must be an int32 vector of odd length on the device of the other tensors")
+    qp, qg = _indices(device, q_pos.shape, q_pos=q_pos, q_group=q_group)
+    kp, kg = _indices(device, k_pos.shape, k_pos=k_pos, k_group=k_group)
+    return qp, kp, lut.contiguous(), qg, kg
+
+
+def padded_planes(b, h, nq, nk, device, dtype):
+    """An uninitialised [b, h, nq, nk] whose rows start on 16-byte boundaries (the layout the attention kernels
+    read fastest): a view of rows padded to a multiple of 8 elements."""
+    return torch.empty(b, h, nq, (nk + 7) // 8 * 8, device=device, dtype=dtype)[..., :nk]
+
+
+def relative_position_bias(table, q_pos, k_pos, lut, q_group=None, k_group=None, out_dtype=None):
+    """Learned relative position bias of attention heads by buckets, [B, H, Nq, Nk].
+
+    ``out[b, h, i, j] = table[u, h]`` with ``u = lut[clip(q_pos[b, i] - k_pos[b, j], -D, D) + D]``, or the last
+    bucket where ``q_group[b, i] != k_group[b, j]`` (other chains, when groups are given).  ``table`` is fp32
+    [buckets, H] (at most 256 buckets); ``lut`` int32 [2 D + 1], see :func:`clipped_buckets` and
+    :func:`log_spaced_buckets` (entries outside the table count as its last bucket); positions and groups are integers
+    [B, Nq] and [B, Nk].  The planes come in ``out_dtype`` (fp32 or bf16, default fp32) with rows on 16-byte boundaries,
+    as :func:`cross_attention` takes them.  Gradient: :func:`relative_position_bias_backward`.
+    """
+    _require_inference(table)
+    _require_cuda(table, q_pos, k_pos, lut)
+    if table.dim() != 2 or table.dtype != torch.float32:
+        raise RuntimeError("table must be fp32 [buckets, heads]")
+    device = table.device
+    qp, kp, lut, qg, kg = _bias_positions(device, q_pos, k_pos, lut, q_group, k_group)
+    (b, nq), nk = qp.shape, kp.shape[1]
+    buckets, h = table.shape
+    out = padded_planes(b, h, nq, nk, device, _float_dtype(out_dtype or torch.float32, "out_dtype"))
+    table = table.contiguous()
+    launch(device, "bl_relative_position_bias", table.data_ptr(), qp.data_ptr(), kp.data_ptr(), lut.data_ptr(),
+           lut.numel() // 2, ptr(qg), ptr(kg), b, h, nq, nk, buckets, out.data_ptr(), _lib.dtype_code(out.dtype),
+           out.stride(0), out.stride(1), out.stride(2))
+    return out
+
+
+def relative_position_bias_backward(grad, q_pos, k_pos, lut, q_group=None, k_group=None, num_buckets=None):
+    """Gradient of :func:`relative_position_bias` with respect to its table: fp32 [num_buckets, H] from the gradient of
+    the planes, fp32 or bf16 [B, H, Nq, Nk] of any strides with contiguous rows.  Sums are fp32 in a fixed order."""
+    _require_inference(grad)
+    _require_cuda(grad, q_pos, k_pos, lut)
+    if grad.dim() != 4 or num_buckets is None:
+        raise RuntimeError("grad must be [B, H, Nq, Nk] and num_buckets be given")
+    _float_dtype(grad.dtype, "grad")
+    device = grad.device
+    qp, kp, lut, qg, kg = _bias_positions(device, q_pos, k_pos, lut, q_group, k_group)
+    b, h, nq, nk = grad.shape
+    if tuple(qp.shape) != (b, nq) or tuple(kp.shape) != (b, nk):
+        raise RuntimeError(f"positions must be [{b}, {nq}] and [{b}, {nk}]")
+    if grad.stride(3) != 1:
+        grad = grad.contiguous()
+    dtable = torch.empty(num_buckets, h, device=device, dtype=torch.float32)
+    nbytes = size_of("bl_relative_position_bias_workspace", b, h, nq, nk, num_buckets)
+    work = _workspace(nbytes, device)
+    launch(device, "bl_relative_position_bias_backward", grad.data_ptr(), _lib.dtype_code(grad.dtype), grad.stride(0),
+           grad.stride(1), grad.stride(2), qp.data_ptr(), kp.data_ptr(), lut.data_ptr(), lut.numel() // 2, ptr(qg), ptr(kg),
+           b, h, nq, nk, num_buckets, dtable.data_ptr(), work.data_ptr(), nbytes)
+    return dtable

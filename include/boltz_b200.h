@@ -7,7 +7,8 @@
  * calling thread).  No entry point allocates device memory: intermediate
  * buffers are passed in by the caller, except for bl_pair_transition_static,
  * whose intermediates live in a fixed array compiled into the library (see
- * its declaration).  Inference only: nothing here records autograd state.
+ * its declaration).  Nothing here records autograd state; the operators with
+ * a gradient have a backward entry of their own.
  *
  * Each declaration names the reference interface it replaces
  * (lauritsf/boltz-lumi, path relative to src/boltz_lumi/).
@@ -401,6 +402,61 @@ BL_API int bl_diffusion_epilogue_split3(const float *a, const float *b, const fl
 BL_API int bl_pair_transition_static(const float *x, int64_t rows, const float *ln_weight,
                                      const float *ln_bias, float eps, const void *w12, const void *w3,
                                      void *out, void *stream);
+
+/*
+ * Relative position encoding of a pair tensor (AF3 supplementary Algorithm 3):
+ *   out[b][i][j] = W[:, p] + W[:, R + t] + [entity_i == entity_j] W[:, 2 R] + W[:, 2 R + 1 + c],  R = 2 r_max + 2
+ *   p = clip(residue_i - residue_j + r_max, 0, 2 r_max)  if asym_i == asym_j, else 2 r_max + 1
+ *   t = clip(token_i - token_j + r_max, 0, 2 r_max)      if also residue_i == residue_j, else 2 r_max + 1
+ *   c = 2 s_max + 1 if asym_i == asym_j (fix_sym: if entity_i != entity_j),
+ *       else clip(sym_i - sym_j + s_max, 0, 2 s_max)
+ * weight: fp32 [channels][2 R + 1 + 2 s_max + 2] (upstream RelativePositionEncoder's
+ * linear_layer.weight); the five token features: int64 [batch][n]; out: fp32
+ * or bf16 [batch][n][n][channels], 16-byte aligned; add != 0 (fp32 only) adds
+ * to what out holds.  channels: a multiple of 4, at most 4096; r_max <= 96,
+ * s_max <= 16, n <= 32768.  No counterpart in the reference, which leaves
+ * upstream's one-hot features and linear in place.
+ * The backward entry sums the upstream gradient (fp32 or bf16
+ * [batch][n][n][channels]) into dweight (fp32, laid out as weight, overwritten);
+ * workspace: at least bl_relative_position_encoding_workspace(...) bytes.
+ * The same inputs give the same bits.
+ */
+BL_API int bl_relative_position_encoding(const float *weight, const int64_t *residue, const int64_t *asym,
+                                         const int64_t *entity, const int64_t *token, const int64_t *sym,
+                                         int64_t batch, int64_t n, int64_t channels, int64_t r_max, int64_t s_max,
+                                         int fix_sym, void *out, int out_dtype, int add, void *stream);
+BL_API int64_t bl_relative_position_encoding_workspace(int64_t batch, int64_t n, int64_t channels, int64_t r_max,
+                                                       int64_t s_max);
+BL_API int bl_relative_position_encoding_backward(const void *grad, int dtype, const int64_t *residue,
+                                                  const int64_t *asym, const int64_t *entity, const int64_t *token,
+                                                  const int64_t *sym, int64_t batch, int64_t n, int64_t channels,
+                                                  int64_t r_max, int64_t s_max, int fix_sym, float *dweight,
+                                                  void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Learned relative position bias of attention heads by buckets:
+ *   out[b][h][i][j] = table[u][h],  u = lut[clip(q_pos[b][i] - k_pos[b][j], -distance, distance) + distance],
+ *   u = buckets - 1 where q_group[b][i] != k_group[b][j]  (groups NULL: all the same)
+ * table: fp32 [buckets][heads]; lut: int32 [2 * distance + 1] (an entry outside
+ * [0, buckets) counts as the last bucket); positions and groups: int64 [batch][nq] /
+ * [batch][nk]; out: fp32 or bf16, element (b, h, i, j) at b*sb + h*sh + i*sq + j
+ * (only these are written).  heads <= 1024, buckets <= 256, heads * buckets <= 40960,
+ * distance <= 8192.  No counterpart in the reference.
+ * The backward entry sums the gradient of the planes (same layout) into dtable
+ * (fp32 [buckets][heads], overwritten); workspace as above.  The same inputs
+ * give the same bits.
+ */
+BL_API int bl_relative_position_bias(const float *table, const int64_t *q_pos, const int64_t *k_pos, const int *lut,
+                                     int64_t distance, const int64_t *q_group, const int64_t *k_group, int64_t batch,
+                                     int64_t heads, int64_t nq, int64_t nk, int64_t buckets, void *out, int out_dtype,
+                                     int64_t sb, int64_t sh, int64_t sq, void *stream);
+BL_API int64_t bl_relative_position_bias_workspace(int64_t batch, int64_t heads, int64_t nq, int64_t nk,
+                                                   int64_t buckets);
+BL_API int bl_relative_position_bias_backward(const void *grad, int dtype, int64_t sb, int64_t sh, int64_t sq,
+                                              const int64_t *q_pos, const int64_t *k_pos, const int *lut,
+                                              int64_t distance, const int64_t *q_group, const int64_t *k_group,
+                                              int64_t batch, int64_t heads, int64_t nq, int64_t nk, int64_t buckets,
+                                              float *dtable, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
