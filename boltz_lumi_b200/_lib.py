@@ -20,6 +20,20 @@ BL_EPI_MODULATION, BL_EPI_GATE, BL_EPI_GATED_SWIGLU, BL_EPI_SWIGLU = 0, 1, 3, 2
 _p = c_void_p
 _i64p = ctypes.POINTER(c_int64)
 
+
+
+class CrossAttentionArgs(ctypes.Structure):
+    """``bl_cross_attention_args``."""
+
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "gate", "bias", "mask")]
+                + [(n, c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "gate_stride", "bias_stride")]
+                + [(n, c_int64) for n in ("mask_stride", "bias_share", "batch", "heads", "kv_heads", "nq", "nk", "head_dim")]
+                + [("out", c_void_p), ("low", c_void_p), ("lse", c_void_p), ("scale", c_float), ("inf", c_float), ("dtype", c_int),
+                   ("mask_kind", c_int)])
+
+
+_xargs = ctypes.POINTER(CrossAttentionArgs)
+
 # name -> argument types (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
     "bl_last_error": [],
@@ -65,8 +79,12 @@ SIGNATURES = {
     "bl_relative_position_bias_workspace": [c_int64] * 5,
     "bl_relative_position_bias_backward": [_p, c_int] + [c_int64] * 3 + [_p] * 3 + [c_int64, _p, _p] + [c_int64] * 5
                                           + [_p, _p, c_int64, _p],
+    "bl_cross_attention": [_xargs, _p],
+    "bl_cross_attention_workspace": [_xargs],
+    "bl_cross_attention_backward": [_xargs] + [_p] * 5 + [c_int64, _p, _p, c_int64, _p],
 }
-_RESTYPES = {"bl_last_error": ctypes.c_char_p, "bl_relative_position_encoding_workspace": c_int64,
+_RESTYPES = {"bl_last_error": ctypes.c_char_p, "bl_cross_attention_workspace": c_int64,
+             "bl_relative_position_encoding_workspace": c_int64,
              "bl_relative_position_bias_workspace": c_int64}
 
 _lib = None

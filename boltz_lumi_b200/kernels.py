@@ -9,6 +9,7 @@ no fallback path.
 
 import functools
 import math
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -578,3 +579,152 @@ def relative_position_bias_backward(grad, q_pos, k_pos, lut, q_group=None, k_gro
            grad.stride(1), grad.stride(2), qp.data_ptr(), kp.data_ptr(), lut.data_ptr(), lut.numel() // 2, ptr(qg), ptr(kg),
            b, h, nq, nk, num_buckets, dtable.data_ptr(), work.data_ptr(), nbytes)
     return dtable
+
+
+# ---------------------------------------------------------------------------
+# Cross attention to states of another length
+# ---------------------------------------------------------------------------
+def _attention_rows(t, dtype, name, shape):
+    """A [B, N, H, d] operand whose rows the kernels can read in place, copied only if they cannot."""
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    sb, si, sh, sd = t.stride()
+    vec = 16 // t.element_size()
+    if sd != 1 or sb % vec or si % vec or sh % vec or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _attention_args(q, k, v, bias, mask, inf, gate, scale):
+    """(the filled argument structure, the tensors it points into)."""
+    device = _require_cuda(q, k, v, bias, mask, gate)
+    if q.dim() != 4 or k.dim() != 4:
+        raise RuntimeError("q must be [B, Nq, H, d], k and v [B, Nk, Hk, d]")
+    b, nq, h, d = q.shape
+    nk, hk = k.shape[1], k.shape[2]
+    dtype = _float_dtype(q.dtype, "q")
+    if hk < 1 or h % hk:
+        raise RuntimeError(f"{hk} key/value heads must divide the {h} query heads")
+    if d % 8 or not 8 <= d <= 128:
+        raise RuntimeError(f"head_dim must be a multiple of 8, at most 128, got {d}")
+    q = _attention_rows(q, dtype, "q", (b, nq, h, d))
+    k = _attention_rows(k, dtype, "k", (b, nk, hk, d))
+    v = _attention_rows(v, dtype, "v", (b, nk, hk, d))
+    x = _lib.CrossAttentionArgs()
+    x.q, x.k, x.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    x.q_stride[:], x.k_stride[:], x.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    if gate is not None:
+        gate = _attention_rows(gate, dtype, "gate", (b, nq, h, d))
+        x.gate = gate.data_ptr()
+        x.gate_stride[:] = gate.stride()[:3]
+    x.bias_share = 1
+    if bias is not None:
+        if bias.dtype != dtype or bias.dim() != 4 or tuple(bias.shape[1:]) != (h, nq, nk) or bias.shape[0] < 1 \
+                or b % bias.shape[0]:
+            raise RuntimeError(f"bias must be {dtype} [B', {h}, {nq}, {nk}] with B' dividing {b}, got {bias.dtype} "
+                               f"{list(bias.shape)}")
+        if bias.stride(3) != 1 and nk > 1:
+            planes = padded_planes(*bias.shape, device, dtype)
+            bias = planes.copy_(bias)
+        x.bias = bias.data_ptr()
+        x.bias_stride[:] = bias.stride()[:3]
+        x.bias_share = b // bias.shape[0]
+    if mask is not None:
+        if tuple(mask.shape) != (b, nk):
+            raise RuntimeError(f"mask must be [{b}, {nk}], got {list(mask.shape)}")
+        if inf is None:
+            if mask.dtype != torch.bool:
+                raise RuntimeError("a mask without inf must be bool (True: the key is kept)")
+            x.mask_kind = 1
+        else:
+            mask = mask.float()
+            x.mask_kind, x.inf = 2, float(inf)
+        if mask.stride(1) != 1 and nk > 1:
+            mask = mask.contiguous()
+        x.mask, x.mask_stride = mask.data_ptr(), mask.stride(0)
+    x.batch, x.heads, x.kv_heads, x.nq, x.nk, x.head_dim = b, h, hk, nq, nk, d
+    x.scale = d ** -0.5 if scale is None else float(scale)
+    x.dtype = _lib.dtype_code(dtype)
+    return x, (q, k, v, bias, mask, gate)
+
+
+class AttentionStats(NamedTuple):
+    """What :func:`cross_attention_backward` takes from the forward call besides its output."""
+
+    rows: torch.Tensor  # fp32 [2, B, H, Nq]: maximum of a row's scores (-inf: no keys), log of the sum relative to it
+    low: Optional[torch.Tensor]  # bf16 [B, Nq, H, d]: what rounding took from the output; None for fp32
+
+
+def cross_attention(q, k, v, bias=None, mask=None, inf=None, gate=None, scale=None, return_lse=False):
+    """Attention of Nq queries to Nk states: ``sigmoid(gate) * softmax(q k^T * scale + bias + mask term) v``.
+
+    ``q`` (and the gate logits ``gate``) are [B, Nq, H, d], ``k`` and ``v`` [B, Nk, Hk, d] with Hk dividing H (head
+    ``h`` reads key/value head ``h // (H / Hk)``); d a multiple of 8, at most 128; all fp32 or all bf16, any strides
+    (copied only if the rows do not start on 16-byte boundaries), so overlapping windows of one tensor are a view.
+    ``bias``: [B', H, Nq, Nk] of the same dtype, B' dividing B (sample ``b`` reads bias ``b // (B / B')``), fastest with
+    rows on 16-byte boundaries (:func:`padded_planes`, :func:`relative_position_bias`).  ``mask`` [B, Nk]: bool, False
+    keys are left out whatever they hold; or, with ``inf``, any real mask added as ``inf * (mask - 1)`` (upstream
+    AttentionPairBias).  ``scale`` defaults to d ** -0.5.  A query whose keys are all left out gets zeros.
+
+    Scores, softmax statistics and sums are fp32; bf16 probabilities are rounded to bf16 for the product with ``v``.
+    Returns [B, Nq, H, d], with ``return_lse`` also the :class:`AttentionStats` that :func:`cross_attention_backward`
+    takes (``rows.sum(0)`` is the log-sum-exp of the scores).
+    """
+    _require_inference(q, k, v, bias, gate)
+    x, kept = _attention_args(q, k, v, bias, mask, inf, gate, scale)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    x.out = out.data_ptr()
+    lse = None
+    if return_lse:
+        rows = torch.empty(2, x.batch, x.heads, x.nq, device=q.device, dtype=torch.float32)
+        low = torch.empty_like(out) if out.dtype == torch.bfloat16 else None
+        lse = AttentionStats(rows, low)
+        x.lse, x.low = rows.data_ptr(), ptr(low)
+    launch(q.device, "bl_cross_attention", x)
+    del kept
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_backward(grad, q, k, v, out, lse, bias=None, mask=None, inf=None, gate=None, scale=None,
+                             need_bias_grad=True):
+    """Gradients of :func:`cross_attention`: (dq, dk, dv, dbias, dgate), None where there is no such input.
+
+    ``grad`` is the gradient of ``out``; the other arguments are the forward call's, ``out`` and ``lse`` (an
+    :class:`AttentionStats`) its results.
+    ``dk`` and ``dv`` are summed over the query heads that share a key/value head and ``dbias`` ([B', H, Nq, Nk], rows on
+    16-byte boundaries) over the samples that share a bias, in fp32 and in a fixed order: the same inputs give the same
+    bits.  The mask is a constant.  ``need_bias_grad=False`` skips dbias.
+    """
+    _require_inference(grad, q, k, v, bias, gate)
+    x, kept = _attention_args(q, k, v, bias, mask, inf, gate, scale)
+    b, nq, h, d = q.shape
+    device, dtype = q.device, q.dtype
+    for name, t in (("grad", grad), ("out", out)):
+        if tuple(t.shape) != (b, nq, h, d) or t.dtype != dtype or t.device != device:
+            raise RuntimeError(f"{name} must be {dtype} {[b, nq, h, d]} on {device}")
+    rows, low = lse
+    if rows.dtype != torch.float32 or tuple(rows.shape) != (2, b, h, nq) or not rows.is_contiguous() \
+            or rows.device != device:
+        raise RuntimeError("lse must be the forward call's statistics (contiguous fp32 rows [2, B, H, Nq])")
+    if low is not None and (low.shape != out.shape or low.dtype != torch.bfloat16 or dtype != torch.bfloat16
+                            or not low.is_contiguous() or low.data_ptr() % 16 or low.device != device):
+        raise RuntimeError("lse.low must be the forward call's contiguous bf16 [B, Nq, H, d]")
+    grad, out = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+                 for t in (grad, out))
+    x.out, x.lse, x.low = out.data_ptr(), rows.data_ptr(), ptr(low)
+    dq = torch.empty(b, nq, h, d, device=device, dtype=dtype)
+    dk = torch.empty(k.shape, device=device, dtype=dtype)
+    dv = torch.empty(k.shape, device=device, dtype=dtype)
+    dgate = None if gate is None else torch.empty(b, nq, h, d, device=device, dtype=dtype)
+    dbias, ld = None, 0
+    if bias is not None and need_bias_grad:
+        dbias = padded_planes(*bias.shape, device, dtype)
+        ld = (x.nk + 7) // 8 * 8
+    nbytes = size_of("bl_cross_attention_workspace", x)
+    work = _workspace(nbytes, device)
+    launch(device, "bl_cross_attention_backward", x, grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+           ptr(dbias), ld, ptr(dgate), work.data_ptr(), nbytes)
+    del kept
+    return dq, dk, dv, dbias, dgate

@@ -458,6 +458,56 @@ BL_API int bl_relative_position_bias_backward(const void *grad, int dtype, int64
                                               int64_t batch, int64_t heads, int64_t nq, int64_t nk, int64_t buckets,
                                               float *dtable, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * Cross attention of nq queries to nk states, with an additive bias, a key mask
+ * and a sigmoid output gate:
+ *   x = (q[b][i][h] . k[b][j][h']) * scale + bias[b / bias_share][h][i][j] + mask term,   h' = h / (heads / kv_heads)
+ *   out[b][i][h] = sigmoid(gate[b][i][h]) * sum_j softmax_j(x) v[b][j][h']
+ * q, k, v, gate, bias and out are all fp32 or all bf16 (dtype); sums, maxima and
+ * softmax statistics are fp32.  q / gate element (b, i, h, e) at b*stride[0] +
+ * i*stride[1] + h*stride[2] + e, k / v likewise; rows on 16-byte boundaries.
+ * bias (NULL: none): element (b', h, i, j) at b'*stride[0] + h*stride[1] +
+ * i*stride[2] + j; one bias serves bias_share consecutive samples.
+ * mask_kind 0: none; 1: uint8 [batch][nk], keys with 0 are left out, whatever
+ * their k, v and bias hold; 2: fp32 [batch][nk], x += inf * (mask - 1).
+ * A query whose keys are all left out (mask, -inf bias or nk = 0) gets 0.
+ * gate may be NULL; out: [batch][nq][heads][head_dim] contiguous; lse (NULL:
+ * not wanted): fp32 [2][batch][heads][nq], the row maximum of x (-inf for a query
+ * without keys) and the log of the sum of exp(x - maximum); low (bf16 only, NULL:
+ * not wanted): bf16 like out, the part of the result that rounding took from out,
+ * which keeps the gradients of rows with one dominant key exact.  head_dim: a multiple of 8, at most 128.
+ * The reference runs the atom transformer's attention (32 queries to 128 keys)
+ * through upstream's eager code; its self-attention form is pair_bias.py:28-36.
+ */
+typedef struct bl_cross_attention_args {
+  const void *q, *k, *v, *gate, *bias, *mask;
+  int64_t q_stride[3], k_stride[3], v_stride[3], gate_stride[3], bias_stride[3];
+  int64_t mask_stride, bias_share;
+  int64_t batch, heads, kv_heads, nq, nk, head_dim;
+  void *out, *low;
+  float *lse;
+  float scale, inf;
+  int dtype, mask_kind;
+} bl_cross_attention_args;
+
+BL_API int bl_cross_attention(const bl_cross_attention_args *args, void *stream);
+
+/*
+ * Gradients of bl_cross_attention: args as in the forward call (out, lse and low: what it
+ * wrote; low may be NULL), dy the gradient of out ([batch][nq][heads][head_dim] contiguous).  Writes
+ * dq and dgate (like out; dgate only with a gate), dk and dv ([batch][nk][kv_heads]
+ * [head_dim] contiguous, summed over the heads that share them) and, unless NULL,
+ * dbias ([batch / bias_share][heads][nq] rows of dbias_ld elements, summed over the
+ * samples that share it; dbias_ld a multiple of 8), all of args' dtype and 16-byte
+ * aligned.  Left-out keys and queries without keys get 0.  workspace: at least
+ * bl_cross_attention_workspace(args) bytes, 16-byte aligned.  No atomics: the same
+ * inputs give the same bits.
+ */
+BL_API int64_t bl_cross_attention_workspace(const bl_cross_attention_args *args);
+BL_API int bl_cross_attention_backward(const bl_cross_attention_args *args, const void *dy, void *dq, void *dk, void *dv,
+                                       void *dbias, int64_t dbias_ld, void *dgate, void *workspace,
+                                       int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
