@@ -14,6 +14,8 @@
 // Both forwards are bound by their HBM writes and both gradients by reading
 // the upstream gradient once.  The gradients are deterministic: every partial
 // sum belongs to one thread, and partials are added in a fixed order.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace bl {
@@ -48,18 +50,26 @@ __device__ __forceinline__ uint32_t pick(const EncArgs &a, int64_t i, int64_t j)
   return p | (t << 10) | (c << 20) | (uint32_t(agree) << 30);
 }
 
-// W[c0 .. c0 + kC)[rows] -> shared [rows][kC + 4].  Eight lanes read eight
-// consecutive columns of one W row (a full 32-byte sector), four rows per
-// warp step; the padded row makes the 32 transposed stores conflict-free
-// ((4 row + c) mod 32 are distinct).
+// W[c0 .. c0 + kC)[rows] -> shared [rows][kC + 4], by 4-byte asynchronous copies: all of a
+// thread's are in flight at once (a load-store loop took 40 of 63 us at 512 tokens).  Eight
+// lanes read eight consecutive columns of one W row (a full 32-byte sector), four rows
+// per warp step; the padded row keeps the 32 transposed writes in distinct banks.
 template <int kC> __device__ __forceinline__ void load_rows(float *dst, const float *w, const EncArgs &a, int c0) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int groups = (a.rows + 7) / 8;
-  for (int u = warp; u < groups * (kC / 4); u += warps) {
-    const int row = (u % groups) * 8 + (lane & 7), c = (u / groups) * 4 + (lane >> 3);
-    if (row < a.rows)
-      dst[row * (kC + 4) + c] = c0 + c < a.channels ? w[int64_t(c0 + c) * a.rows + row] : 0.f;
+  const int c = lane >> 3;
+  for (int r0 = 0; r0 < a.rows; r0 += 8) {
+    const int row = r0 + (lane & 7);
+    for (int q = warp; q < kC / 4; q += warps) {
+      const bool ok = row < a.rows && c0 + 4 * q + c < a.channels;
+      if (row < a.rows) {
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst + row * (kC + 4) + 4 * q + c));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to),
+                     "l"(w + (ok ? int64_t(c0 + 4 * q + c) * a.rows + row : 0)), "r"(ok ? 4 : 0)
+                     : "memory");
+      }
+    }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
@@ -83,14 +93,14 @@ __global__ void __launch_bounds__(256) encoding_kernel(const float *w, const Enc
   const int sub = lane / kLanes, c = 4 * (lane % kLanes);
   const int n = a.n, segments = (n + 31) / 32;
   const bool live = c0 + c < a.channels;
-  const int64_t units = a.batch * n * segments;
+  const uint32_t units = uint32_t(a.batch * n * segments);  // below 2^31: checked by the host
   const float *col = rows + c;
   uint32_t held = 0xffffffffu;
   float4 base = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int64_t u = int64_t(blockIdx.x) * warps + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * warps) {
-    const int64_t i = u / segments;  // b * n + row
-    const int j0 = int(u % segments) * 32;
-    const int64_t b0 = i / n * n;
+  for (uint32_t u = blockIdx.x * warps + (threadIdx.x >> 5); u < units; u += gridDim.x * warps) {
+    const uint32_t row = u / uint32_t(segments);  // b * n + i
+    const int j0 = int(u - row * segments) * 32;
+    const int64_t i = row, b0 = row / uint32_t(n) * n;
     const uint32_t mine = j0 + lane < n ? pick(a, i, b0 + j0 + lane) : 0u;
     const int count = n - j0 < 32 ? n - j0 : 32;
     Out *dst = out + (i * n + j0) * a.channels + c0 + c;
@@ -118,99 +128,91 @@ __global__ void __launch_bounds__(256) encoding_kernel(const float *w, const Enc
   }
 }
 
-// Gradient of W.  A group of warps covers kC = 128 channels (fp32: four warps
-// of one channel per lane; bf16: two warps of two channels per lane) and owns
+// Gradient of W.  A group of two warps covers 128 channels (two per lane) and owns
 // a private [rows][128] table in shared memory, each element of which one lane
 // alone updates.  A group walks diagonals: from pair (i0, j) it visits
-// (i0 + s, (j + s) mod n) for kSteps rows, every load a coalesced part of a
-// pair row.  Along a diagonal of one chain the offsets, so the picks, do not
-// change: the sums stay in registers and reach the table when a pick changes.
-constexpr int kSteps = 32;
+// (i0 + s, (j + s) mod n) for up to kSteps rows, every load a coalesced half of a
+// pair row, all of a walk's loads in flight at once.  Along a diagonal of one chain
+// the offsets, so the picks, do not change: the sum of the pairs stays in registers
+// and goes to the table rows of its picks when one of them changes.
 constexpr int kGroups = 3;  // private tables per CTA (71 KB each at r = 32, s = 2)
+template <typename In> constexpr int kSteps = sizeof(In) == 4 ? 32 : 64;
 
 template <typename In>
-__global__ void __launch_bounds__(kGroups * 128) encoding_grad_kernel(const In *grad, const EncArgs a,
-                                                                     float *partial) {
-  constexpr int kPer = sizeof(In) == 4 ? 1 : 2;  // channels per lane
-  constexpr int kWarps = 4 / kPer;               // warps per group
+__global__ void __launch_bounds__(kGroups * 64) encoding_grad_kernel(const In *grad, const EncArgs a, float *partial) {
+  constexpr int kS = kSteps<In>;
   extern __shared__ float4 smem4[];
   float *tables = reinterpret_cast<float *>(smem4);
-  const int groups = blockDim.x / (32 * kWarps);
-  const int size = a.rows * 128;
-  for (int i = threadIdx.x; i < groups * size; i += blockDim.x) tables[i] = 0.f;
+  const int groups = blockDim.x / 64, size = a.rows * 128;
+  for (int i = threadIdx.x; i < groups * size / 4; i += blockDim.x) smem4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = warp / kWarps, ch = (warp % kWarps) * 32 * kPer + lane * kPer, c0 = blockIdx.y * 128;
+  const int lane = threadIdx.x & 31, group = threadIdx.x / 64;
+  const int ch = threadIdx.x % 64 * 2, c0 = blockIdx.y * 128;
   const bool live = c0 + ch < a.channels;  // channels is even
-  float *mine = tables + group * size + ch;
-  const int n = a.n, blocks = (n + kSteps - 1) / kSteps;
-  const int64_t units = a.batch * blocks * n;
-  float run_p[kPer], run_t[kPer], run_c[kPer], run_e[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) run_p[e] = run_t[e] = run_c[e] = run_e[e] = 0.f;
+  float2 *mine = reinterpret_cast<float2 *>(tables + group * size + ch);
+  const int n = a.n, blocks = (n + kS - 1) / kS;
+  const uint32_t units = uint32_t(a.batch * blocks * n);
+  const int64_t step = (int64_t(n) + 1) * a.channels, wrap = int64_t(n) * a.channels;
+  float2 run = make_float2(0.f, 0.f);
   uint32_t held = 0xffffffffu;
-  auto put = [&](uint32_t row, float (&run)[kPer]) {
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) mine[row * 128 + e] += run[e], run[e] = 0.f;
+  auto put = [&](uint32_t row) {
+    float2 v = mine[row * 64];
+    v.x += run.x, v.y += run.y;
+    mine[row * 64] = v;
   };
-  auto change = [&](uint32_t v) {  // warp-uniform
-    const uint32_t was = held;
-    held = v;
-    if (was == 0xffffffffu) return;
-    if ((was ^ v) & 1023u) put(was & 1023u, run_p);
-    if ((was ^ v) & (1023u << 10)) put((was >> 10) & 1023u, run_t);
-    if ((was ^ v) & (1023u << 20)) put((was >> 20) & 1023u, run_c);
+  auto flush = [&]() {
+    put(held & 1023u), put((held >> 10) & 1023u), put((held >> 20) & 1023u);
+    if (held >> 30) put(4 * a.r + 4);
+    run = make_float2(0.f, 0.f);
   };
-  const int64_t stride = int64_t(gridDim.x) * groups;
-  for (int64_t u = int64_t(blockIdx.x) * groups + group; u < units; u += stride) {
-    const int j = int(u % n);
-    const int64_t ib = u / n;
-    const int i0 = int(ib % blocks) * kSteps;
-    const int64_t b0 = ib / blocks * n;
-    const int count = n - i0 < kSteps ? n - i0 : kSteps;
-    uint32_t packed = 0;
-    if (lane < count) packed = pick(a, b0 + i0 + lane, b0 + (j + lane) % n);
-    float x[kSteps][kPer];
+  for (uint32_t u = blockIdx.x * groups + group; u < units; u += gridDim.x * groups) {
+    const uint32_t ib = u / uint32_t(n), b = ib / uint32_t(blocks);
+    const int j = int(u - ib * n), i0 = int(ib - b * blocks) * kS;
+    const int64_t b0 = int64_t(b) * n;
+    const int count = n - i0 < kS ? n - i0 : kS;
+    const In *p = grad + ((b0 + i0) * n + j) * a.channels + c0 + ch;
+    typename std::conditional<sizeof(In) == 4, float2, uint32_t>::type x[kS];
+    int col = j;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) x[s][e] = 0.f;
+    for (int s = 0; s < kS; ++s) {
       if (s < count && live) {
-        int col = j + s;
-        while (col >= n) col -= n;
-        const In *p = grad + ((b0 + i0 + s) * n + col) * a.channels + c0 + ch;
-        if constexpr (kPer == 1) {
-          x[s][0] = __ldcs(p);
-        } else {
-          const uint32_t v = __ldcs(reinterpret_cast<const unsigned int *>(p));
-          x[s][0] = bf16_lo(v), x[s][1] = bf16_hi(v);
-        }
+        if constexpr (sizeof(In) == 4)
+          x[s] = __ldcs(reinterpret_cast<const float2 *>(p));
+        else
+          x[s] = __ldcs(reinterpret_cast<const unsigned int *>(p));
+      } else {
+        x[s] = {};
       }
+      p += step;
+      if (++col == n) col = 0, p -= wrap;
+    }
+    uint32_t packed[kS / 32];
+#pragma unroll
+    for (int e = 0; e < kS / 32; ++e) {
+      const int s = 32 * e + lane;
+      packed[e] = s < count ? pick(a, b0 + i0 + s, b0 + (j + s) % n) : 0u;
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
+    for (int s = 0; s < kS; ++s) {
       if (s >= count) break;
-      const uint32_t v = __shfl_sync(0xffffffffu, packed, s);
-      if (v != held) change(v);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        run_p[e] += x[s][e], run_t[e] += x[s][e], run_c[e] += x[s][e];
-        if (v >> 30) run_e[e] += x[s][e];
+      const uint32_t v = __shfl_sync(0xffffffffu, packed[s / 32], s % 32);
+      if (v != held) {
+        if (held != 0xffffffffu) flush();
+        held = v;
       }
+      if constexpr (sizeof(In) == 4)
+        run.x += x[s].x, run.y += x[s].y;
+      else
+        run.x += bf16_lo(x[s]), run.y += bf16_hi(x[s]);
     }
   }
-  if (held != 0xffffffffu) {
-    put(held & 1023u, run_p);
-    put((held >> 10) & 1023u, run_t);
-    put((held >> 20) & 1023u, run_c);
-    put(4 * a.r + 4, run_e);
-  }
+  if (held != 0xffffffffu) flush();
   __syncthreads();
   // partial[cta][channel chunk][row][128]
-  float *dst = partial + (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * size;
-  for (int i = threadIdx.x; i < size; i += blockDim.x) {
-    float v = tables[i];
-    for (int g = 1; g < groups; ++g) v += tables[g * size + i];
+  float4 *dst = reinterpret_cast<float4 *>(partial + (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * size);
+  for (int i = threadIdx.x; i < size / 4; i += blockDim.x) {
+    float4 v = smem4[i];
+    for (int g = 1; g < groups; ++g) v = add4(v, smem4[g * (size / 4) + i]);
     dst[i] = v;
   }
 }
@@ -236,6 +238,7 @@ __global__ void __launch_bounds__(256) encoding_grad_sum_kernel(const float *par
 
 int encoding_check(const char *name, const EncArgs &a, int64_t n, int64_t channels, int64_t r, int64_t s) {
   BL_REQUIRE(a.batch >= 0 && n >= 0 && n <= (1 << 15) && a.batch <= (1 << 20), "%s: bad shape", name);
+  BL_REQUIRE(a.batch * n * ((n + 31) / 32) < (int64_t(1) << 31), "%s: too many token pairs", name);
   BL_REQUIRE(channels >= 4 && channels <= 4096 && channels % 4 == 0, "%s: channels must be a multiple of 4, at most 4096",
              name);
   BL_REQUIRE(r >= 0 && s >= 0 && r <= 96 && s <= 16, "%s: r_max must lie in [0, 96], s_max in [0, 16]", name);
@@ -248,7 +251,7 @@ int encoding_grad_groups(int rows) {  // private tables that fit in 227 KB
   return fit < kGroups ? fit : kGroups;
 }
 int64_t encoding_grad_ctas(int64_t batch, int64_t n, int rows, int chunks) {
-  const int64_t units = batch * ((n + kSteps - 1) / kSteps) * n, groups = encoding_grad_groups(rows);
+  const int64_t units = batch * ((n + 31) / 32) * n, groups = encoding_grad_groups(rows);
   const int64_t want = (units + groups - 1) / groups, cap = (num_sms() + chunks - 1) / chunks;
   return want < 1 ? 1 : want < cap ? want : cap;
 }
@@ -327,6 +330,32 @@ __global__ void __launch_bounds__(kBiasThreads) bias_kernel(const float *table, 
   }
 }
 
+// Four neighbouring elements of a row as loaded.
+template <typename T> struct Quad;
+template <> struct Quad<float> {
+  using type = float4;
+  static __device__ __forceinline__ float4 load(const float *p, int count, bool vector) {
+    if (vector) return __ldcs(reinterpret_cast<const float4 *>(p));
+    return make_float4(p[0], count > 1 ? p[1] : 0.f, count > 2 ? p[2] : 0.f, count > 3 ? p[3] : 0.f);
+  }
+  static __device__ __forceinline__ float get(const float4 &v, int e) {
+    return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+  }
+};
+template <> struct Quad<__nv_bfloat16> {
+  using type = uint2;
+  static __device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, int count, bool vector) {
+    if (vector) return __ldcs(reinterpret_cast<const uint2 *>(p));
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < count ? __bfloat162float(p[e]) : 0.f;
+    return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));  // exact
+  }
+  static __device__ __forceinline__ float get(const uint2 &v, int e) {
+    return e == 0 ? bf16_lo(v.x) : e == 1 ? bf16_hi(v.x) : e == 2 ? bf16_lo(v.y) : bf16_hi(v.y);
+  }
+};
+
 // Gradient of the table.  A thread owns four key columns of kHeads heads and
 // walks down the query rows with one running sum per column and head; when a
 // column's bucket changes, its sums go to the thread's own column of the
@@ -343,13 +372,16 @@ __global__ void __launch_bounds__(kBiasThreads) bias_grad_kernel(const In *grad,
   __syncthreads();
   float *mine = hist + threadIdx.x;
   const int h0 = blockIdx.y * kHeads, heads = a.heads - h0 < kHeads ? a.heads - h0 : kHeads;
-  const int col_blocks = (a.nk + kBiasCols - 1) / kBiasCols, row_blocks = (a.nq + q_rows - 1) / q_rows;
-  const int64_t units = a.batch * col_blocks * row_blocks;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int j = int(u % col_blocks) * kBiasCols + 4 * int(threadIdx.x);
-    if (j >= a.nk) continue;
-    const int64_t rb = u / col_blocks, b = rb / row_blocks;
-    const int i0 = int(rb % row_blocks) * q_rows, i1 = i0 + q_rows < a.nq ? i0 + q_rows : a.nq;
+  // Four columns per thread, consecutive over all samples: no thread idles at a row's end.
+  const int quads = (a.nk + 3) / 4, row_blocks = (a.nq + q_rows - 1) / q_rows;
+  const uint32_t all_quads = uint32_t(a.batch * quads), col_blocks = (all_quads + kBiasThreads - 1) / kBiasThreads;
+  const uint32_t units = col_blocks * row_blocks;
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const uint32_t rb = u / col_blocks, quad = (u - rb * col_blocks) * kBiasThreads + threadIdx.x;
+    if (quad >= all_quads) continue;
+    const int64_t b = quad / uint32_t(quads);
+    const int j = 4 * int(quad - uint32_t(b) * quads);
+    const int i0 = int(rb) * q_rows, i1 = i0 + q_rows < a.nq ? i0 + q_rows : a.nq;
     const int count = a.nk - j < 4 ? a.nk - j : 4;
     int64_t kp[4], kg[4];
     int held[4];
@@ -364,30 +396,14 @@ __global__ void __launch_bounds__(kBiasThreads) bias_grad_kernel(const In *grad,
       for (int h = 0; h < kHeads; ++h) run[e][h] = 0.f;
     }
     const In *base = grad + b * a.sb + h0 * a.sh + j;
-#pragma unroll 2
-    for (int i = i0; i < i1; ++i) {
-      float x[kHeads][4];
+    auto load = [&](int i, typename Quad<In>::type (&x)[kHeads]) {
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[h][e] = 0.f;
-        if (h < heads) {
-          const In *p = base + h * a.sh + int64_t(i) * a.sq;
-          if (vector && count == 4) {
-            if constexpr (sizeof(In) == 4) {
-              const float4 v = __ldcs(reinterpret_cast<const float4 *>(p));
-              x[h][0] = v.x, x[h][1] = v.y, x[h][2] = v.z, x[h][3] = v.w;
-            } else {
-              const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(p));
-              x[h][0] = bf16_lo(v.x), x[h][1] = bf16_hi(v.x), x[h][2] = bf16_lo(v.y), x[h][3] = bf16_hi(v.y);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (e < count) x[h][e] = load_as_float(p + e);
-          }
-        }
+        x[h] = {};
+        if (h < heads) x[h] = Quad<In>::load(base + h * a.sh + int64_t(i) * a.sq, count, vector && count == 4);
       }
+    };
+    auto take = [&](int i, const typename Quad<In>::type (&x)[kHeads]) {
       const int64_t qp = a.q_pos[b * a.nq + i], qg = a.q_group ? a.q_group[b * a.nq + i] : 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -403,8 +419,22 @@ __global__ void __launch_bounds__(kBiasThreads) bias_grad_kernel(const In *grad,
           held[e] = v;
         }
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) run[e][h] += x[h][e];
+        for (int h = 0; h < kHeads; ++h) run[e][h] += Quad<In>::get(x[h], e);
       }
+    };
+    constexpr int kAhead = 4;  // rows in flight
+    int i = i0;
+    for (; i + kAhead <= i1; i += kAhead) {
+      typename Quad<In>::type x[kAhead][kHeads];
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) load(i + r, x[r]);
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) take(i + r, x[r]);
+    }
+    for (; i < i1; ++i) {
+      typename Quad<In>::type x[kHeads];
+      load(i, x);
+      take(i, x);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -444,18 +474,31 @@ int bias_check(const char *name, const BiasArgs &a) {
   BL_REQUIRE(int64_t(a.heads) * a.buckets <= 40960, "%s: heads * buckets must be at most 40960", name);
   BL_REQUIRE(a.lut, "%s: lut is required", name);
   BL_REQUIRE(a.batch == 0 || a.nq == 0 || a.nk == 0 || (a.q_pos && a.k_pos), "%s: positions are required", name);
+  BL_REQUIRE(a.batch * ((a.nk + 3) / 4) * int64_t(a.nq) < (int64_t(1) << 38) && a.batch * a.nk < (int64_t(1) << 31),
+             "%s: shape too large", name);
   BL_REQUIRE(!a.q_group == !a.k_group, "%s: give both groups or neither", name);
   return BL_OK;
 }
 
 int bias_lut_bytes(int distance) { return (2 * distance + 1) * 2; }
 int bias_grad_heads(int buckets) { return buckets <= 48 ? 4 : 1; }  // 2 KB (4 heads) or 0.5 KB (1) per bucket
-int bias_grad_rows(int64_t nq) { return nq < 64 ? int(nq < 1 ? 1 : nq) : 64; }
-int64_t bias_grad_ctas(int64_t batch, int heads, int64_t nq, int64_t nk, int buckets) {
-  const int per = bias_grad_heads(buckets), rows = bias_grad_rows(nq);
-  const int64_t units = batch * ((nk + kBiasCols - 1) / kBiasCols) * ((nq + rows - 1) / rows);
-  const int64_t groups = (heads + per - 1) / per, cap = (2 * num_sms() + groups - 1) / groups;
-  return units < 1 ? 1 : units < cap ? units : cap;
+// Launch shape of the table gradient: three CTAs per SM (67 KB of histogram at 33 buckets x 4 heads), and rows per
+// unit such that a CTA has about eight units to even out, in whole groups of four rows.
+struct BiasGrad {
+  int per, groups, rows;
+  int64_t ctas;
+};
+BiasGrad bias_grad_shape(int64_t batch, int64_t heads, int64_t nq, int64_t nk, int buckets) {
+  BiasGrad g;
+  g.per = bias_grad_heads(buckets);
+  g.groups = int((heads + g.per - 1) / g.per);
+  const int64_t cols = (batch * ((nk + 3) / 4) + kBiasThreads - 1) / kBiasThreads;
+  const int64_t cap = (3 * num_sms() + g.groups - 1) / g.groups;
+  int64_t rows = nq * cols / (8 * cap) / 4 * 4;
+  g.rows = int(rows < 4 ? 4 : rows > 64 ? 64 : rows);
+  const int64_t units = cols * ((nq + g.rows - 1) / g.rows);
+  g.ctas = units < 1 ? 1 : units < cap ? units : cap;
+  return g;
 }
 
 bool vector_planes(const void *p, const BiasArgs &a, int dtype) {
@@ -525,9 +568,10 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
     BL_CUDA(cudaMemsetAsync(dweight, 0, size_t(channels) * a.rows * 4, st));
     return BL_OK;
   }
-  BL_REQUIRE(grad && aligned_to(grad, 4), "bl_relative_position_encoding_backward: null or unaligned pointer");
+  BL_REQUIRE(grad && aligned_to(grad, dtype == BL_F32 ? 8 : 4),
+             "bl_relative_position_encoding_backward: null or unaligned pointer");
   const int64_t need = bl_relative_position_encoding_workspace(batch, n, channels, r_max, s_max);
-  BL_REQUIRE(workspace && workspace_bytes >= need && aligned_to(workspace, 4),
+  BL_REQUIRE(workspace && workspace_bytes >= need && aligned_to(workspace, 16),
              "bl_relative_position_encoding_backward: needs a workspace of %lld bytes", (long long)need);
   const int chunks = int((channels + 127) / 128), groups = encoding_grad_groups(a.rows);
   const int64_t ctas = encoding_grad_ctas(batch, n, a.rows, chunks);
@@ -536,7 +580,7 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
   dim3 grid{unsigned(ctas), unsigned(chunks)};
   if (dtype == BL_F32) {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(encoding_grad_kernel<float>), kMaxSmem));
-    encoding_grad_kernel<float><<<grid, groups * 128, smem, st>>>(static_cast<const float *>(grad), a, part);
+    encoding_grad_kernel<float><<<grid, groups * 64, smem, st>>>(static_cast<const float *>(grad), a, part);
   } else {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(encoding_grad_kernel<__nv_bfloat16>), kMaxSmem));
     encoding_grad_kernel<__nv_bfloat16>
@@ -586,8 +630,8 @@ extern "C" int bl_relative_position_bias(const float *table, const int64_t *q_po
 extern "C" int64_t bl_relative_position_bias_workspace(int64_t batch, int64_t heads, int64_t nq, int64_t nk,
                                                        int64_t buckets) {
   if (batch <= 0 || heads <= 0 || heads > 1024 || nq <= 0 || nk <= 0 || buckets <= 0 || buckets > 256) return 0;
-  const int64_t per = bias_grad_heads(int(buckets)), groups = (heads + per - 1) / per;
-  return bias_grad_ctas(batch, int(heads), nq, nk, int(buckets)) * groups * buckets * per * 4;
+  const BiasGrad g = bias_grad_shape(batch, heads, nq, nk, int(buckets));
+  return g.ctas * g.groups * buckets * g.per * 4;
 }
 
 extern "C" int bl_relative_position_bias_backward(const void *grad, int dtype, int64_t sb, int64_t sh, int64_t sq,
@@ -611,8 +655,9 @@ extern "C" int bl_relative_position_bias_backward(const void *grad, int dtype, i
   const int64_t need = bl_relative_position_bias_workspace(batch, heads, nq, nk, buckets);
   BL_REQUIRE(grad && workspace && workspace_bytes >= need && aligned_to(workspace, 4),
              "bl_relative_position_bias_backward: needs grad and a workspace of %lld bytes", (long long)need);
-  const int per = bias_grad_heads(a.buckets), groups = (a.heads + per - 1) / per, rows = bias_grad_rows(nq);
-  const int64_t ctas = bias_grad_ctas(batch, a.heads, nq, nk, a.buckets);
+  const BiasGrad shape = bias_grad_shape(batch, heads, nq, nk, a.buckets);
+  const int per = shape.per, groups = shape.groups, rows = shape.rows;
+  const int64_t ctas = shape.ctas;
   const int smem = a.buckets * per * kBiasThreads * 4 + bias_lut_bytes(a.distance);
   float *part = static_cast<float *>(workspace);
   const int vec = vector_planes(grad, a, dtype);
