@@ -446,6 +446,11 @@ template <typename T> int forward(const Args &a, cudaStream_t stream) {
     if (a.d <= 64) return launch_step<T, 64>(a, stream);
     return launch_step<T, 128>(a, stream);
   }
+  if (sizeof(T) == 2) {
+    bool taken = false;
+    if (int rc = forward_tc(a, stream, &taken)) return rc;
+    if (taken) return BL_OK;
+  }
   if (a.d <= 32) return launch_flash<T, 32>(a, stream);
   if (a.d <= 64) return launch_flash<T, 64>(a, stream);
   return launch_flash<T, 128>(a, stream);

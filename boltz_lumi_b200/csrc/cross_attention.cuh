@@ -36,7 +36,7 @@ struct Args {
   int batch, heads, group, nq, nk, d;  // group: query heads per key/value head
   void *out;    // [batch][nq][heads][d]
   void *low;    // like out, or null: what rounding to bf16 took from out, itself rounded to bf16
-  float *lse;   // [2][batch][heads][nq] or null: row maximum, log of the sum relative to it
+  float *lse;   // [2][batch][heads][nq] or null: a reference of the row's scores, log of the sum relative to it
   __host__ __device__ int64_t lse_plane() const { return int64_t(batch) * heads * nq; }
 };
 
@@ -297,6 +297,8 @@ __device__ __forceinline__ void clear_left_out(T *rows, const float *mk, int tid
 // cross_attention.cu
 Args make_args(const bl_cross_attention_args *x);
 int check(const char *name, const Args &a, int64_t kv_heads, int dtype);
+// cross_attention_tc.cu
+int forward_tc(const Args &a, cudaStream_t stream, bool *taken);
 
 }  // namespace xa
 }  // namespace bl

@@ -653,7 +653,7 @@ def _attention_args(q, k, v, bias, mask, inf, gate, scale):
 class AttentionStats(NamedTuple):
     """What :func:`cross_attention_backward` takes from the forward call besides its output."""
 
-    rows: torch.Tensor  # fp32 [2, B, H, Nq]: maximum of a row's scores (-inf: no keys), log of the sum relative to it
+    rows: torch.Tensor  # fp32 [2, B, H, Nq]: reference of a row's scores (-inf: no keys), log of the sum relative to it
     low: Optional[torch.Tensor]  # bf16 [B, Nq, H, d]: what rounding took from the output; None for fp32
 
 

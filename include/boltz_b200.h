@@ -472,8 +472,9 @@ BL_API int bl_relative_position_bias_backward(const void *grad, int dtype, int64
  * their k, v and bias hold; 2: fp32 [batch][nk], x += inf * (mask - 1).
  * A query whose keys are all left out (mask, -inf bias or nk = 0) gets 0.
  * gate may be NULL; out: [batch][nq][heads][head_dim] contiguous; lse (NULL:
- * not wanted): fp32 [2][batch][heads][nq], the row maximum of x (-inf for a query
- * without keys) and the log of the sum of exp(x - maximum); low (bf16 only, NULL:
+ * not wanted): fp32 [2][batch][heads][nq], a reference of the row's scores (their
+ * maximum or a little below it; -inf for a query without keys) and the log of the
+ * sum of exp(x - reference): their sum is the log-sum-exp; low (bf16 only, NULL:
  * not wanted): bf16 like out, the part of the result that rounding took from out,
  * which keeps the gradients of rows with one dominant key exact.  head_dim: a multiple of 8, at most 128.
  * The reference runs the atom transformer's attention (32 queries to 128 keys)
