@@ -1,0 +1,105 @@
+// Parts shared by the tcgen05 cross-attention kernels.
+#pragma once
+
+#include "cross_attention.cuh"
+#include "tc.cuh"
+
+namespace bl {
+namespace xa {
+namespace {
+
+constexpr int kMaskWords = 2048;  // keys whose mask is kept as bits in shared memory, / 32
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_addr(dst)), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// 128-byte swizzle, K-major (LBO unused), 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t(hi) << 32) | lo; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Bounded wait that polls: tc::mbar_wait's timer read and timed suspension lengthen the
+// chain of waits per tile (5 % of the kernel); the timer is read once in 4096 polls.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, unsigned int *status, unsigned code) {
+  uint64_t start = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((spin & 4095u) == 0) {
+      if (*reinterpret_cast<volatile unsigned int *>(status) != 0u) return false;
+      const uint64_t now = tc::global_timer_ns();
+      if (start == 0) start = now;
+      if (now - start > tc::kWaitLimitNs) {
+        atomicCAS(status, 0u, code);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsigned int *status, unsigned code) {
+  return __all_sync(0xffffffffu, wait_phase(bar, parity, status, code));
+}
+
+__device__ __forceinline__ int n_words(int nk) { return (nk + 31) / 32; }
+// Bits of keys [32 w, 32 w + 32): left out by a keep mask, changed by an additive one, or past nk.
+__device__ __forceinline__ uint32_t mask_word(const Args &a, int b, int w) {
+  uint32_t word = 0;
+  const int j0 = 32 * w;
+  if (a.mask_kind == kMaskKeep) {
+    const uint8_t *m = static_cast<const uint8_t *>(a.mask) + b * a.mask_sb + j0;
+    if (j0 + 32 <= a.nk && (reinterpret_cast<uintptr_t>(m) & 15) == 0) {
+      const uint4 v[2] = {reinterpret_cast<const uint4 *>(m)[0], reinterpret_cast<const uint4 *>(m)[1]};
+      const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // 0xff where a byte is zero; its low bits gathered to four
+        word |= ((__vcmpeq4(u[e], 0u) & 0x01010101u) * 0x10204080u >> 28) << (4 * e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) word |= uint32_t(j0 + e >= a.nk || m[e] == 0) << e;
+    }
+  } else {
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) word |= uint32_t(mask_value(a, b, j0 + e) != 0.f) << e;
+  }
+  return word;
+}
+// Map of a [batch][rows][heads][d] view: box of 64 columns x box_rows rows; false where TMA cannot describe it.
+bool rows_map(CUtensorMap *map, const Rows &r, int d, int rows, int heads, int batch, int box_rows) {
+  const int64_t strides[3] = {r.si, r.sh, r.sb};
+  const int sizes[3] = {rows, heads, batch};
+  uint64_t dims[4] = {uint64_t(d), uint64_t(rows), uint64_t(heads), uint64_t(batch)}, bytes[3];
+  for (int e = 0; e < 3; ++e) {
+    if (sizes[e] > 1 && strides[e] <= 0) return false;
+    bytes[e] = sizes[e] > 1 ? uint64_t(strides[e]) * 2 : 16;
+    if (bytes[e] >= (uint64_t(1) << 40)) return false;
+  }
+  const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.p, dims, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace
+}  // namespace xa
+}  // namespace bl
