@@ -15,26 +15,14 @@
 //   queries_kernel one CTA = up to 64 query rows of one (sample, head): dq, and
 //                  dbias where no other sample shares the bias;
 //   bias_kernel    one CTA = one block of a shared bias: dbias summed over its samples.
-#include "cross_attention.cuh"
+#include "cross_attention_backward.cuh"
 
 namespace bl {
 namespace xa {
 namespace {
 
-struct BackArgs {
-  Args a;  // a.out: the forward's output, a.lse: its statistics
-  const void *dy, *dout;  // gradient of out; do ([batch][nq][heads][d]; dy itself without a gate)
-  const void *dlow;       // bf16 with a gate: do - bf16(do), else null
-  float *delta;           // [batch][heads][nq]
-  void *dq, *dk, *dv, *dgate, *dbias;  // contiguous; dbias [batch / share][heads][nq][dbias_ld] or null
-  int64_t dbias_ld;
-};
-
 // Query rows per tile of keys_kernel and key columns per tile of the others.
 template <typename T, int DP> constexpr int kTile = (sizeof(T) == 4 || DP == 128) ? 32 : 64;
-
-// The saved row maximum as grad_score wants it: +inf for a query without keys (all its p become 0).
-__device__ __forceinline__ float row_max(float m) { return m == -INFINITY ? INFINITY : m; }
 
 // p and ds of one score, given the row's maximum m, -log2 of its sum and delta.  m is
 // subtracted before the change of base: in a row of the type's lowest values the sum
@@ -468,7 +456,10 @@ template <typename T, int DP> int launch(const BackArgs &x, cudaStream_t stream)
   BL_REQUIRE(rows_total < (int64_t(1) << 35), "bl_cross_attention_backward: too many query rows");
   rows_kernel<T><<<unsigned((rows_total + 31) / 32), 256, 0, stream>>>(x, rows_total);
   BL_LAUNCH_CHECK();
-  if (a.nk > 0) {
+  bool taken = false;
+  if (sizeof(T) == 2)
+    if (int rc = keys_tc(x, stream, &taken)) return rc;
+  if (a.nk > 0 && !taken) {
     const int64_t tiles = (a.nk + kKeys - 1) / kKeys, ctas = tiles * (a.heads / a.group) * a.batch;
     BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention_backward: too many key tiles");
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(keys_kernel<T, DP>), 232448));
@@ -478,10 +469,19 @@ template <typename T, int DP> int launch(const BackArgs &x, cudaStream_t stream)
   const int warps = a.nq >= 64 ? 4 : (a.nq + 15) / 16, rows = 16 * warps;
   const int64_t tiles = (a.nq + rows - 1) / rows, ctas = tiles * a.heads * a.batch;
   BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention_backward: too many query tiles");
-  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(queries_kernel<T, DP>), 232448));
-  queries_kernel<T, DP><<<unsigned(ctas), 32 * warps, queries_smem<T, DP>(rows, biased, x.dlow != nullptr), stream>>>(x, int(tiles));
-  BL_LAUNCH_CHECK();
-  if (x.dbias && a.share > 1 && a.nk > 0) {
+  taken = false;
+  if (sizeof(T) == 2)
+    if (int rc = queries_tc(x, stream, &taken)) return rc;
+  if (!taken) {
+    BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(queries_kernel<T, DP>), 232448));
+    queries_kernel<T, DP>
+        <<<unsigned(ctas), 32 * warps, queries_smem<T, DP>(rows, biased, x.dlow != nullptr), stream>>>(x, int(tiles));
+    BL_LAUNCH_CHECK();
+  }
+  taken = false;
+  if (sizeof(T) == 2 && x.dbias && a.share > 1)
+    if (int rc = bias_tc(x, stream, &taken)) return rc;
+  if (x.dbias && a.share > 1 && a.nk > 0 && !taken) {
     const int cols = (a.nk + kTile<T, DP> - 1) / kTile<T, DP>;
     const int64_t blocks = tiles * cols * a.heads * (a.batch / a.share);
     BL_REQUIRE(blocks < (int64_t(1) << 31), "bl_cross_attention_backward: too many bias blocks");

@@ -1,0 +1,841 @@
+// Cross attention gradients on tcgen05 tensor cores (bf16; see cross_attention_backward.cu
+// for the formulas).
+//
+//   queries_tc_kernel  one CTA = 128 query rows of one (sample, head) over key tiles of 64:
+//                      S = Q K^T and dP = dO V^T in TMEM, dS = p (dP - delta) as bf16 in TMEM,
+//                      dQ += dS K; dS itself is the bias gradient where no sample shares the bias.
+//   keys_tc_kernel     one CTA = 128 keys of one (sample, key/value head) over query tiles of 64 of
+//                      every head that reads them: S^T = K Q^T and dP^T = V dO^T, P^T and dS^T as
+//                      bf16 in TMEM, dV += P^T dO, dK += dS^T Q.
+//
+// Both: warp 0 feeds the tiles by TMA, warp 1 issues the MMAs, warps 4..11 own half a TMEM lane's
+// columns per thread (lane = the resident row).  A tile's scores go to registers at once, so the
+// next tile's products run under this tile's arithmetic.  There is no row maximum to agree on:
+// the forward's statistics give p directly.  A gated do enters dP as two bf16 terms.
+// Against the same loops on mma.sync (measured in cross_attention_backward.cu's comment) they
+// gain because the 16-row warp products there re-read every operand tile from shared memory
+// once per 16 rows.
+#include "cross_attention_backward.cuh"
+#include "cross_attention_tc.cuh"
+
+namespace bl {
+namespace xa {
+namespace {
+
+constexpr int kRowsTc = 128, kTileTc = 64, kThreadsTc = 12 * 32;
+using Bf = __nv_bfloat16;
+
+struct BackTc {
+  BackArgs x;
+  int tiles;  // resident row tiles per (sample, head)
+  unsigned int *status;
+};
+
+template <int kBlocks, bool kBias, bool kLow> struct QShape {
+  static constexpr int kRes = kRowsTc * 128 * kBlocks;  // bytes of a resident 128-row tile
+  static constexpr int kStr = kTileTc * 128 * kBlocks;  // bytes of a streamed 64-row tile
+  static constexpr int kB = kBias ? kRowsTc * kTileTc * 2 : 0;
+  static constexpr int kStages = kBlocks == 2 && kLow && kBias ? 2 : 3, kBiasStages = 2;
+  static constexpr int kResident = kLow ? 3 : 2;        // Q, dO, do - bf16(do)
+  static constexpr int kStrOff = kResident * kRes;      // [stage]{K, V}
+  static constexpr int kBiasOff = kStrOff + kStages * 2 * kStr;
+  static constexpr int kMaskOff = kBiasOff + kBiasStages * kB;  // [warp][32] additive mask values
+  static constexpr int kBitsOff = kMaskOff + 8 * 32 * 4;
+  static constexpr int kBarOff = kBitsOff + kMaskWords * 4;
+  static constexpr int kBytes = kBarOff + 256 + 1024;
+};
+// TMEM columns: S, dP (64 each), two dS buffers (32 each), dQ.
+constexpr uint32_t kSCol = 0, kDpCol = 64, kDsCol = 128, kDqCol = 256;
+
+template <int kBlocks, bool kBias, bool kLow>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    queries_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                      const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias,
+                      const BackTc p) {
+  using S = QShape<kBlocks, kBias, kLow>;
+  constexpr int ST = S::kStages, BS = S::kBiasStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
+  uint64_t *res_full = bars;             // resident tiles landed
+  uint64_t *st_full = res_full + 1;      // [ST] K and V of a key tile landed
+  uint64_t *st_empty = st_full + ST;     // [ST] dQ has read that K
+  uint64_t *b_full = st_empty + ST;      // [BS] bias block landed
+  uint64_t *b_empty = b_full + BS;       // [BS] it has been read
+  uint64_t *s_full = b_empty + BS;       // S and dP in TMEM
+  uint64_t *s_free = s_full + 1;         // they are in registers
+  uint64_t *ds_full = s_free + 1;        // [2] dS in TMEM
+  uint64_t *dq_full = ds_full + 2;       // every product is done
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(dq_full + 1);
+  int *last_key = reinterpret_cast<int *>(tmem_slot + 1);
+  const Args &a = p.x.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int tile, h, b;
+  decode_cta(a, blockIdx.x, p.tiles, a.heads, tile, h, b);
+  const int q0 = tile * kRowsTc, hk = h / a.group, bb = b / a.share;
+  if (tid == 0) {
+    tc::mbar_init(res_full, 1);
+    for (int i = 0; i < ST; ++i) tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1);
+    for (int i = 0; i < BS; ++i) tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 8);
+    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8), tc::mbar_init(dq_full, 1);
+    tc::mbar_init(ds_full, 8), tc::mbar_init(ds_full + 1, 8);
+    tc::fence_mbar_init();
+    *last_key = -1;
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  uint32_t *bits = reinterpret_cast<uint32_t *>(smem + S::kBitsOff);
+  const bool use_bits = a.nk <= 32 * kMaskWords;
+  int keys = a.nk;
+  if (a.mask_kind != kMaskNone && use_bits) {
+    int best = -1;
+    for (int w = tid; w < (n_words(a.nk) + 1) / 2 * 2; w += kThreadsTc) {
+      const uint32_t word = mask_word(a, b, w);
+      bits[w] = word;
+      if (word != 0xffffffffu) best = 32 * w + 31 - __clz(~word);
+    }
+    if (a.mask_kind == kMaskKeep && best >= 0) atomicMax(last_key, best);
+    __syncthreads();
+    // Key tiles past the last kept key add nothing to dq; where dbias is written here they are
+    // visited all the same, to write their zeros.
+    if (a.mask_kind == kMaskKeep && !(kBias && p.x.dbias && a.share == 1)) keys = *last_key + 1;
+  }
+  const int n = (keys + kTileTc - 1) / kTileTc;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      tc::mbar_arrive_expect_tx(res_full, S::kResident * S::kRes);
+      for (int c = 0; c < kBlocks; ++c) {
+        tma_load_4d(smem + c * kRowsTc * 128, &map_q, res_full, 64 * c, q0, h, b);
+        tma_load_4d(smem + S::kRes + c * kRowsTc * 128, &map_do, res_full, 64 * c, q0, h, b);
+        if (kLow) tma_load_4d(smem + 2 * S::kRes + c * kRowsTc * 128, &map_low, res_full, 64 * c, q0, h, b);
+      }
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const int s = j % ST;
+        if (j >= ST && !(ok = wait_phase(st_empty + s, ((j / ST) & 1) ^ 1u, p.status, 0x401))) break;
+        uint8_t *st = smem + S::kStrOff + s * 2 * S::kStr;
+        tc::mbar_arrive_expect_tx(st_full + s, 2 * S::kStr);
+        for (int c = 0; c < kBlocks; ++c) {
+          tma_load_4d(st + c * kTileTc * 128, &map_k, st_full + s, 64 * c, j * kTileTc, hk, b);
+          tma_load_4d(st + S::kStr + c * kTileTc * 128, &map_v, st_full + s, 64 * c, j * kTileTc, hk, b);
+        }
+        if constexpr (kBias) {
+          const int bs = j % BS;
+          if (j >= BS && !(ok = wait_phase(b_empty + bs, ((j / BS) & 1) ^ 1u, p.status, 0x402))) break;
+          tc::mbar_arrive_expect_tx(b_full + bs, S::kB);
+          tma_load_4d(smem + S::kBiasOff + bs * S::kB, &map_bias, b_full + bs, j * kTileTc, q0, h, bb);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0 && wait_phase(res_full, 0, p.status, 0x403)) {
+      constexpr uint32_t idesc_s = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
+      const int steps = (a.d + 15) / 16;
+      const uint32_t idesc_dq = tc::idesc_bf16(kRowsTc, 16 * steps, false, true);
+      const uint32_t base = smem_addr(smem);
+      auto product = [&](uint32_t col, uint32_t res, uint32_t str, bool add) {  // resident rows . streamed rows
+        for (int e = 0; e < steps; ++e)
+          tc::umma_f16_ss(tmem + col, desc_k(res + (e >> 2) * kRowsTc * 128 + (e & 3) * 32),
+                          desc_k(str + (e >> 2) * kTileTc * 128 + (e & 3) * 32), idesc_s, add || e != 0);
+      };
+      auto issue = [&](int j) {
+        const int s = j % ST;
+        if (!wait_phase(st_full + s, (j / ST) & 1, p.status, 0x404)) return false;
+        if (j > 0 && !wait_phase(s_free, (j - 1) & 1, p.status, 0x405)) return false;
+        tc::tc_fence_after();
+        const uint32_t k = base + S::kStrOff + s * 2 * S::kStr, v = k + S::kStr;
+        product(kSCol, base, k, false);
+        product(kDpCol, base + S::kRes, v, false);
+        if (kLow) product(kDpCol, base + 2 * S::kRes, v, true);
+        tc::umma_commit(s_full);
+        return true;
+      };
+      bool ok = issue(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n && !(ok = issue(j + 1))) break;
+        if (!(ok = wait_phase(ds_full + (j & 1), (j >> 1) & 1, p.status, 0x406))) break;
+        tc::tc_fence_after();
+        const uint32_t k = base + S::kStrOff + (j % ST) * 2 * S::kStr;
+#pragma unroll
+        for (int e = 0; e < kTileTc / 16; ++e)
+          tc::umma_f16_ts(tmem + kDqCol, tmem + kDsCol + (j & 1) * 32 + e * 8, tc::desc_sw128(k + e * 2048, kTileTc * 128),
+                          idesc_dq, (j | e) != 0);
+        tc::umma_commit(st_empty + j % ST);
+        if (j + 1 == n) tc::umma_commit(dq_full);
+      }
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = q0 + row;
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+    float *mk = reinterpret_cast<float *>(smem + S::kMaskOff) + (warp - 4) * 32;
+    float m = INFINITY, nl = 0.f, delta = 0.f;
+    if (i < a.nq) {
+      const int64_t at = (int64_t(b) * a.heads + h) * a.nq + i;
+      m = row_max(a.lse[at]), nl = -kLog2e * a.lse[a.lse_plane() + at], delta = p.x.delta[at];
+    }
+    // A reference of the type's lowest values overflows in base 2: subtract it first there.
+    const bool lowest = __any_sync(0xffffffffu, m < -1e37f);
+    const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta), scale2 = dup2(a.scale);
+    const uint64_t log2e2 = dup2(kLog2e);
+    Bf *dbias = kBias && p.x.dbias && a.share == 1 && i < a.nq
+                    ? static_cast<Bf *>(p.x.dbias) + ((int64_t(b) * a.heads + h) * a.nq + i) * p.x.dbias_ld
+                    : nullptr;
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      const int k0 = j * kTileTc + 32 * half;
+      uint32_t cut = 0;
+      if (a.mask_kind == kMaskNone) {
+        const int left = a.nk - k0;
+        if (left < 32) cut = left <= 0 ? ~0u : ~0u << left;
+      } else if (use_bits) {
+        cut = bits[2 * j + half];
+      } else {
+        cut = __ballot_sync(0xffffffffu, mask_value(a, b, k0 + lane) != 0.f);
+      }
+      const bool adds = cut && a.mask_kind == kMaskAdd;
+      if (adds) {
+        const float v = mask_value(a, b, k0 + lane);
+        __syncwarp();
+        mk[lane] = v == -INFINITY ? 0.f : v;
+        cut = __ballot_sync(0xffffffffu, v == -INFINITY);  // from here on: keys that count nothing
+        __syncwarp();
+      }
+      if (!(ok = warp_wait(s_full, j & 1, p.status, 0x407))) break;
+      tc::tc_fence_after();
+      uint32_t sv[32], dv[32];
+      tc::tmem_ld_32x32b_x32(lanes + kSCol + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(lanes + kDpCol + 32 * half, dv);
+      const int bs = j % BS;
+      if constexpr (kBias) ok = warp_wait(b_full + bs, (j / BS) & 1, p.status, 0x408);
+      tc::tmem_ld_wait_regs(sv, dv);
+      if (!ok) break;
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(s_free);
+      uint64_t y[16];
+      if constexpr (kBias) {
+        const uint32_t brow = smem_addr(smem + S::kBiasOff + bs * S::kB) + row * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 v = lds128(brow + (((4 * half + c) ^ (row & 7)) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            y[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(b_empty + bs);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
+      }
+      if (adds)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = add2(y[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
+      uint32_t ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        uint64_t z;
+        if (lowest)
+          z = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
+        else
+          z = fma2(y[e], log2e2, c2);
+        const uint64_t prob = pack2(__float_as_uint(fast_exp2(lo_f(z))), __float_as_uint(fast_exp2(hi_f(z))));
+        const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
+        ds[e] = pack_bf16x2(lo_f(g), hi_f(g));
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t c = cut >> (2 * e);
+          ds[e] &= (c & 1 ? 0u : 0xffffu) | (c & 2 ? 0u : 0xffff0000u);
+        }
+        // K rows of left-out keys must be zero before dS meets them in dQ.
+        if (a.mask_kind == kMaskKeep) {
+          const int s = j % ST, key = 8 * quarter + (lane >> 2);
+          if (cut >> key & 1) {
+            wait_phase(st_full + s, (j / ST) & 1, p.status, 0x409);  // complete: S came from this stage
+            uint8_t *k = smem + S::kStrOff + s * 2 * S::kStr + (32 * half + key) * 128 + (lane & 3) * 32;
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint4 *>(k + c * kTileTc * 128 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          tc::fence_proxy_async_smem();
+        }
+      }
+      // dS of tile j - 2 was in this buffer; its dQ product was issued before S of this tile.
+      tc::tmem_st_32x32b_x16(lanes + kDsCol + (j & 1) * 32 + 16 * half, ds);
+      if (kBias && dbias) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int k = k0 + 8 * c;
+          if (k + 8 <= a.nk)
+            *reinterpret_cast<uint4 *>(dbias + k) = make_uint4(ds[4 * c], ds[4 * c + 1], ds[4 * c + 2], ds[4 * c + 3]);
+          else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (k + e < a.nk) reinterpret_cast<uint16_t *>(dbias)[k + e] = uint16_t(ds[4 * c + (e >> 1)] >> (16 * (e & 1)));
+        }
+      }
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(ds_full + (j & 1));
+    }
+    if (ok && n > 0) ok = warp_wait(dq_full, 0, p.status, 0x40A);
+    tc::tc_fence_after();
+    if (ok) {
+      Bf *dq = static_cast<Bf *>(p.x.dq) + ((int64_t(b) * a.nq + i) * a.heads + h) * a.d;
+      for (int c = half; c < (a.d + 15) / 16; c += 2) {
+        uint32_t o[16];
+        if (n > 0) {
+          tc::tmem_ld_32x32b_x16(lanes + kDqCol + 16 * c, o);
+          tc::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e8 = 0; e8 < 2; ++e8) {
+          const int c0 = 16 * c + 8 * e8;
+          if (i >= a.nq || c0 >= a.d) continue;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = n > 0 ? pack_bf16x2(__uint_as_float(o[8 * e8 + 2 * e]) * a.scale, __uint_as_float(o[8 * e8 + 2 * e + 1]) * a.scale)
+                         : 0u;
+          *reinterpret_cast<uint4 *>(dq + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int kBlocks, bool kBias, bool kLow> struct KShape {
+  static constexpr int kRes = kRowsTc * 128 * kBlocks, kStr = kTileTc * 128 * kBlocks;
+  static constexpr int kPer = kLow ? 3 : 2;  // streamed tiles: Q, dO, do - bf16(do)
+  static constexpr int kB = kBias ? kTileTc * kRowsTc * 2 : 0;
+  static constexpr int kStages = kBlocks == 2 ? (kLow ? 2 : 3) : 3;
+  static constexpr int kStrOff = 2 * kRes;  // K, V
+  static constexpr int kBiasOff = kStrOff + kStages * kPer * kStr;
+  static constexpr int kStatOff = kBiasOff + kStages * kB;  // [stage]{reference, -log2 sum, base-2 offset, -delta}[64]
+  static constexpr int kBarOff = kStatOff + kStages * 4 * kTileTc * 4 + kStages * 16;
+  static constexpr int kBytes = kBarOff + 256 + 1024;
+};
+// TMEM columns: S^T, dP^T (64 each), two buffers of P^T and of dS^T (32 each), dV, dK.
+constexpr uint32_t kPtCol = 128, kDstCol = 192, kDvCol = 256, kDkCol = 384;
+
+template <int kBlocks, bool kBias, bool kLow>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    keys_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                   const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias, const BackTc p) {
+  using S = KShape<kBlocks, kBias, kLow>;
+  constexpr int ST = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
+  uint64_t *res_full = bars;             // K and V landed
+  uint64_t *st_full = res_full + 1;      // [ST] Q, dO and the bias block of a query tile landed
+  uint64_t *st_empty = st_full + ST;     // [ST] dV and dK have read them
+  uint64_t *stat_full = st_empty + ST;   // [ST] the rows' statistics are in shared memory
+  uint64_t *stat_empty = stat_full + ST; // [ST] they (and the bias block) have been read
+  uint64_t *s_full = stat_empty + ST;    // S^T and dP^T in TMEM
+  uint64_t *s_free = s_full + 1;         // they are in registers
+  uint64_t *ps_full = s_free + 1;        // [2] P^T and dS^T in TMEM
+  uint64_t *d_full = ps_full + 2;        // every product is done
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_full + 1);
+  float *stats = reinterpret_cast<float *>(smem + S::kStatOff);
+  int *lowest_flag = reinterpret_cast<int *>(stats + ST * 4 * kTileTc);  // [ST], 16 bytes apart
+  const Args &a = p.x.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv_heads = a.heads / a.group;
+  int tile, hk, b;
+  decode_cta(a, blockIdx.x, p.tiles, kv_heads, tile, hk, b);
+  const int j0 = tile * kRowsTc, bb = b / a.share;
+  if (tid == 0) {
+    tc::mbar_init(res_full, 1);
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1);
+      tc::mbar_init(stat_full + i, 1), tc::mbar_init(stat_empty + i, 8);
+    }
+    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8), tc::mbar_init(d_full, 1);
+    tc::mbar_init(ps_full, 8), tc::mbar_init(ps_full + 1, 8);
+    tc::fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, 512);
+    tc::tmem_relinquish();
+  }
+  const bool keeps = tid < kRowsTc && mask_value(a, b, j0 + tid) != -INFINITY;
+  tc::tc_fence_before();
+  const bool any = __syncthreads_or(keeps);
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int q_tiles = (a.nq + kTileTc - 1) / kTileTc, n = any ? q_tiles * a.group : 0;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      tc::mbar_arrive_expect_tx(res_full, 2 * S::kRes);
+      for (int c = 0; c < kBlocks; ++c) {
+        tma_load_4d(smem + c * kRowsTc * 128, &map_k, res_full, 64 * c, j0, hk, b);
+        tma_load_4d(smem + S::kRes + c * kRowsTc * 128, &map_v, res_full, 64 * c, j0, hk, b);
+      }
+      for (int u = 0; u < n; ++u) {
+        const int s = u % ST, h = hk * a.group + u / q_tiles, i0 = u % q_tiles * kTileTc;
+        if (u >= ST && !wait_phase(st_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x411)) break;
+        if (kBias && u >= ST && !wait_phase(stat_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x412)) break;
+        uint8_t *st = smem + S::kStrOff + s * S::kPer * S::kStr;
+        tc::mbar_arrive_expect_tx(st_full + s, S::kPer * S::kStr + S::kB);
+        for (int c = 0; c < kBlocks; ++c) {
+          tma_load_4d(st + c * kTileTc * 128, &map_q, st_full + s, 64 * c, i0, h, b);
+          tma_load_4d(st + S::kStr + c * kTileTc * 128, &map_do, st_full + s, 64 * c, i0, h, b);
+          if (kLow) tma_load_4d(st + 2 * S::kStr + c * kTileTc * 128, &map_low, st_full + s, 64 * c, i0, h, b);
+        }
+        if constexpr (kBias)  // two blocks of 64 keys
+          for (int c = 0; c < 2; ++c)
+            tma_load_4d(smem + S::kBiasOff + s * S::kB + c * kTileTc * 128, &map_bias, st_full + s, j0 + 64 * c, i0, h, bb);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0 && wait_phase(res_full, 0, p.status, 0x413)) {
+      constexpr uint32_t idesc_s = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
+      const int steps = (a.d + 15) / 16;
+      const uint32_t idesc_d = tc::idesc_bf16(kRowsTc, 16 * steps, false, true);
+      const uint32_t base = smem_addr(smem);
+      auto product = [&](uint32_t col, uint32_t res, uint32_t str, bool add) {
+        for (int e = 0; e < steps; ++e)
+          tc::umma_f16_ss(tmem + col, desc_k(res + (e >> 2) * kRowsTc * 128 + (e & 3) * 32),
+                          desc_k(str + (e >> 2) * kTileTc * 128 + (e & 3) * 32), idesc_s, add || e != 0);
+      };
+      auto issue = [&](int u) {
+        const int s = u % ST;
+        if (!wait_phase(st_full + s, (u / ST) & 1, p.status, 0x414)) return false;
+        if (u > 0 && !wait_phase(s_free, (u - 1) & 1, p.status, 0x415)) return false;
+        tc::tc_fence_after();
+        const uint32_t q = base + S::kStrOff + s * S::kPer * S::kStr;
+        product(kSCol, base, q, false);
+        product(kDpCol, base + S::kRes, q + S::kStr, false);
+        if (kLow) product(kDpCol, base + S::kRes, q + 2 * S::kStr, true);
+        tc::umma_commit(s_full);
+        return true;
+      };
+      bool ok = issue(0);
+      for (int u = 0; u < n && ok; ++u) {
+        if (u + 1 < n && !(ok = issue(u + 1))) break;
+        if (!(ok = wait_phase(ps_full + (u & 1), (u >> 1) & 1, p.status, 0x416))) break;
+        tc::tc_fence_after();
+        const uint32_t q = base + S::kStrOff + (u % ST) * S::kPer * S::kStr, d = q + S::kStr;
+#pragma unroll
+        for (int e = 0; e < kTileTc / 16; ++e)
+          tc::umma_f16_ts(tmem + kDvCol, tmem + kPtCol + (u & 1) * 32 + e * 8, tc::desc_sw128(d + e * 2048, kTileTc * 128),
+                          idesc_d, (u | e) != 0);
+#pragma unroll
+        for (int e = 0; e < kTileTc / 16; ++e)
+          tc::umma_f16_ts(tmem + kDkCol, tmem + kDstCol + (u & 1) * 32 + e * 8, tc::desc_sw128(q + e * 2048, kTileTc * 128),
+                          idesc_d, (u | e) != 0);
+        tc::umma_commit(st_empty + u % ST);
+        if (u + 1 == n) tc::umma_commit(d_full);
+      }
+    }
+  } else if (warp == 2) {
+    // ---------------- statistics of the query rows, a tile at a time ----------------
+    for (int u = 0; u < n; ++u) {
+      const int s = u % ST, h = hk * a.group + u / q_tiles, i0 = u % q_tiles * kTileTc;
+      float m[2], nl[2], dl[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = i0 + lane + 32 * e;
+        const int64_t at = (int64_t(b) * a.heads + h) * a.nq + i;
+        m[e] = i < a.nq ? row_max(a.lse[at]) : INFINITY;
+        nl[e] = i < a.nq ? -kLog2e * a.lse[a.lse_plane() + at] : 0.f;
+        dl[e] = i < a.nq ? -p.x.delta[at] : 0.f;
+      }
+      if (u >= ST && !warp_wait(stat_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x417)) break;
+      float *st = stats + s * 4 * kTileTc;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = lane + 32 * e;
+        st[r] = m[e], st[kTileTc + r] = nl[e], st[3 * kTileTc + r] = dl[e];
+        st[2 * kTileTc + r] = m[e] == INFINITY ? -INFINITY : fmaf(-m[e], kLog2e, nl[e]);
+      }
+      const bool lowest = __any_sync(0xffffffffu, m[0] < -1e37f || m[1] < -1e37f);
+      if (lane == 0) lowest_flag[4 * s] = lowest;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(stat_full + s);
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+    const float mkv = mask_value(a, b, j);
+    const bool out = mkv == -INFINITY;
+    const uint64_t scale2 = dup2(a.scale), log2e2 = dup2(kLog2e), mk2 = dup2(out ? 0.f : mkv);
+    const bool adds = __any_sync(0xffffffffu, !out && mkv != 0.f);
+    bool ok = true;
+    for (int u = 0; u < n && ok; ++u) {
+      const int s = u % ST;
+      if (!(ok = warp_wait(s_full, u & 1, p.status, 0x418))) break;
+      tc::tc_fence_after();
+      uint32_t sv[32], dv[32];
+      tc::tmem_ld_32x32b_x32(lanes + kSCol + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(lanes + kDpCol + 32 * half, dv);
+      ok = warp_wait(stat_full + s, (u / ST) & 1, p.status, 0x419) && (!kBias || warp_wait(st_full + s, (u / ST) & 1, p.status, 0x41A));
+      tc::tmem_ld_wait_regs(sv, dv);
+      if (!ok) break;
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(s_free);
+      const float *st = stats + s * 4 * kTileTc + 32 * half;
+      const bool lowest = lowest_flag[4 * s] != 0;
+      // bias(q, key): 64-key block row / 64, row q of 128 bytes, 16-byte chunk (key / 8) ^ (q & 7).
+      const uint8_t *bias = smem + S::kBiasOff + s * S::kB + (row >> 6) * kTileTc * 128 + 32 * half * 128 + (row & 7) * 2;
+      const int chunk = (row & 63) >> 3;
+      uint32_t pt[16], ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        uint64_t y;
+        if constexpr (kBias) {
+          const uint32_t b0 = *reinterpret_cast<const uint16_t *>(bias + (2 * e) * 128 + ((chunk ^ ((2 * e) & 7)) << 4));
+          const uint32_t b1 = *reinterpret_cast<const uint16_t *>(bias + (2 * e + 1) * 128 + ((chunk ^ ((2 * e + 1) & 7)) << 4));
+          y = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(b0 << 16, b1 << 16));
+        } else {
+          y = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
+        }
+        if (adds) y = add2(y, mk2);
+        uint64_t z;
+        if (lowest)
+          z = pack2(__float_as_uint(fmaf(lo_f(y) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
+                    __float_as_uint(fmaf(hi_f(y) - st[2 * e + 1], kLog2e, st[kTileTc + 2 * e + 1])));
+        else
+          z = fma2(y, log2e2, *reinterpret_cast<const uint64_t *>(st + 2 * kTileTc + 2 * e));
+        const float p0 = fast_exp2(lo_f(z)), p1 = fast_exp2(hi_f(z));
+        const uint64_t prob = pack2(__float_as_uint(p0), __float_as_uint(p1));
+        const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), *reinterpret_cast<const uint64_t *>(st + 3 * kTileTc + 2 * e)));
+        pt[e] = out ? 0u : pack_bf16x2(p0, p1);
+        ds[e] = out ? 0u : pack_bf16x2(lo_f(g), hi_f(g));
+      }
+      // The buffers' last products were issued before S^T of this tile, whose commit covers them.
+      tc::tmem_st_32x32b_x16(lanes + kPtCol + (u & 1) * 32 + 16 * half, pt);
+      tc::tmem_st_32x32b_x16(lanes + kDstCol + (u & 1) * 32 + 16 * half, ds);
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(stat_empty + s);
+        tc::mbar_arrive(ps_full + (u & 1));
+      }
+    }
+    if (ok && n > 0) ok = warp_wait(d_full, 0, p.status, 0x41B);
+    tc::tc_fence_after();
+    if (ok) {
+      const int64_t at = ((int64_t(b) * a.nk + j) * kv_heads + hk) * a.d;
+      for (int c = half; c < (a.d + 15) / 16; c += 2) {
+        uint32_t gv[16], gk[16];
+        if (n > 0) {
+          tc::tmem_ld_32x32b_x16(lanes + kDvCol + 16 * c, gv);
+          tc::tmem_ld_32x32b_x16(lanes + kDkCol + 16 * c, gk);
+          tc::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e8 = 0; e8 < 2; ++e8) {
+          const int c0 = 16 * c + 8 * e8;
+          if (j >= a.nk || c0 >= a.d) continue;
+          uint32_t wv[4], wk[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int o = 8 * e8 + 2 * e;
+            wv[e] = n > 0 ? pack_bf16x2(__uint_as_float(gv[o]), __uint_as_float(gv[o + 1])) : 0u;
+            wk[e] = n > 0 ? pack_bf16x2(__uint_as_float(gk[o]) * a.scale, __uint_as_float(gk[o + 1]) * a.scale) : 0u;
+          }
+          *reinterpret_cast<uint4 *>(static_cast<Bf *>(p.x.dv) + at + c0) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+          *reinterpret_cast<uint4 *>(static_cast<Bf *>(p.x.dk) + at + c0) = make_uint4(wk[0], wk[1], wk[2], wk[3]);
+        }
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Gradient of a bias that several samples share: one CTA = 128 query rows of one (bias, head) over a
+// range of key tiles; for each tile the samples' Q, dO, K and V stream through a two-stage ring and the
+// threads add up dS in registers.  d <= 64 (two 64-column blocks would leave one stage).
+template <bool kLow> struct BShape {
+  static constexpr int kRes = kRowsTc * 128, kStr = kTileTc * 128, kPer = kLow ? 3 : 2;
+  static constexpr int kStage = kPer * kRes + 2 * kStr;  // Q, dO, do - bf16(do), K, V
+  static constexpr int kB = kRowsTc * kTileTc * 2;
+  static constexpr int kBiasOff = 2 * kStage, kMaskOff = kBiasOff + 2 * kB, kBarOff = kMaskOff + 8 * 32 * 4;
+  static constexpr int kBytes = kBarOff + 256 + 1024;
+};
+
+template <bool kLow>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    bias_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                   const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias, const BackTc p,
+                   int ranges) {
+  using S = BShape<kLow>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
+  uint64_t *st_full = bars, *st_empty = bars + 2;   // [2] a sample's tiles landed; its products are done
+  uint64_t *b_full = bars + 4, *b_empty = bars + 6; // [2] bias block landed; it has been read
+  uint64_t *s_full = bars + 8, *s_free = bars + 9;  // S and dP in TMEM; in registers
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10);
+  const Args &a = p.x.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int64_t at = blockIdx.x;
+  const int range = int(at % ranges);
+  at /= ranges;
+  const int q0 = int(at % p.tiles) * kRowsTc;
+  at /= p.tiles;
+  const int h = int(at % a.heads), bb = int(at / a.heads), hk = h / a.group;
+  const int key_tiles = (a.nk + kTileTc - 1) / kTileTc;
+  const int t0 = int(int64_t(range) * key_tiles / ranges), t1 = int(int64_t(range + 1) * key_tiles / ranges);
+  const int n = (t1 - t0) * a.share;  // (key tile, sample) steps
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i)
+      tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1), tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 8);
+    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8);
+    tc::fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, 128);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp == 0) {
+    if (lane == 0)
+      for (int u = 0; u < n; ++u) {
+        const int s = u & 1, jt = u / a.share, b = bb * a.share + u % a.share, j0 = (t0 + jt) * kTileTc;
+        if (u >= 2 && !wait_phase(st_empty + s, ((u >> 1) & 1) ^ 1u, p.status, 0x421)) break;
+        uint8_t *st = smem + s * S::kStage;
+        tc::mbar_arrive_expect_tx(st_full + s, S::kStage);
+        tma_load_4d(st, &map_q, st_full + s, 0, q0, h, b);
+        tma_load_4d(st + S::kRes, &map_do, st_full + s, 0, q0, h, b);
+        if (kLow) tma_load_4d(st + 2 * S::kRes, &map_low, st_full + s, 0, q0, h, b);
+        tma_load_4d(st + S::kPer * S::kRes, &map_k, st_full + s, 0, j0, hk, b);
+        tma_load_4d(st + S::kPer * S::kRes + S::kStr, &map_v, st_full + s, 0, j0, hk, b);
+        if (u % a.share == 0) {
+          const int bs = jt & 1;
+          if (jt >= 2 && !wait_phase(b_empty + bs, ((jt >> 1) & 1) ^ 1u, p.status, 0x422)) break;
+          tc::mbar_arrive_expect_tx(b_full + bs, S::kB);
+          tma_load_4d(smem + S::kBiasOff + bs * S::kB, &map_bias, b_full + bs, j0, q0, h, bb);
+        }
+      }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
+      const int steps = (a.d + 15) / 16;
+      for (int u = 0; u < n; ++u) {
+        const int s = u & 1;
+        if (!wait_phase(st_full + s, (u >> 1) & 1, p.status, 0x423)) break;
+        if (u > 0 && !wait_phase(s_free, (u - 1) & 1, p.status, 0x424)) break;
+        tc::tc_fence_after();
+        const uint32_t q = smem_addr(smem) + s * S::kStage, k = q + S::kPer * S::kRes;
+        for (int e = 0; e < steps; ++e) tc::umma_f16_ss(tmem, desc_k(q + e * 32), desc_k(k + e * 32), idesc, e != 0);
+        for (int t = 1; t < S::kPer; ++t)
+          for (int e = 0; e < steps; ++e)
+            tc::umma_f16_ss(tmem + 64, desc_k(q + t * S::kRes + e * 32), desc_k(k + S::kStr + e * 32), idesc, t > 1 || e != 0);
+        tc::umma_commit(s_full);
+        tc::umma_commit(st_empty + s);
+      }
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = q0 + row;
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+    float *mk = reinterpret_cast<float *>(smem + S::kMaskOff) + (warp - 4) * 32;
+    const uint64_t scale2 = dup2(a.scale), log2e2 = dup2(kLog2e);
+    uint64_t acc[16];
+    for (int u = 0; u < n; ++u) {
+      const int jt = u / a.share, first = u % a.share == 0, b = bb * a.share + u % a.share;
+      const int k0 = (t0 + jt) * kTileTc + 32 * half;
+      float m = INFINITY, nl = 0.f, delta = 0.f;
+      if (i < a.nq) {
+        const int64_t r = (int64_t(b) * a.heads + h) * a.nq + i;
+        m = row_max(a.lse[r]), nl = -kLog2e * a.lse[a.lse_plane() + r], delta = p.x.delta[r];
+      }
+      const float mv = mask_value(a, b, k0 + lane);
+      const bool adds = __any_sync(0xffffffffu, mv != 0.f && mv != -INFINITY);
+      const uint32_t cut = __ballot_sync(0xffffffffu, mv == -INFINITY);
+      if (adds) {
+        __syncwarp();
+        mk[lane] = mv == -INFINITY ? 0.f : mv;
+        __syncwarp();
+      }
+      const bool lowest = __any_sync(0xffffffffu, m < -1e37f);
+      if (!warp_wait(s_full, u & 1, p.status, 0x425)) break;
+      tc::tc_fence_after();
+      uint32_t sv[32], dv[32];
+      tc::tmem_ld_32x32b_x32(lanes + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(lanes + 64 + 32 * half, dv);
+      const bool ok = !first || warp_wait(b_full + (jt & 1), (jt >> 1) & 1, p.status, 0x426);
+      tc::tmem_ld_wait_regs(sv, dv);
+      if (!ok) break;
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(s_free);
+      const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta);
+      const uint32_t brow = smem_addr(smem + S::kBiasOff + (jt & 1) * S::kB) + row * 128;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 v = lds128(brow + (((4 * half + c) ^ (row & 7)) << 4));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int e = 4 * c + e4;
+          uint64_t y = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(w[e4] << 16, w[e4] & 0xffff0000u));
+          if (adds) y = add2(y, *reinterpret_cast<const uint64_t *>(mk + 2 * e));
+          uint64_t z;
+          if (lowest)
+            z = pack2(__float_as_uint(fmaf(lo_f(y) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y) - m, kLog2e, nl)));
+          else
+            z = fma2(y, log2e2, c2);
+          uint64_t g = mul2(pack2(__float_as_uint(fast_exp2(lo_f(z))), __float_as_uint(fast_exp2(hi_f(z)))),
+                            add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
+          const uint32_t out = cut >> (2 * e);
+          if (cut) g = pack2(out & 1 ? 0u : uint32_t(g), out & 2 ? 0u : uint32_t(g >> 32));
+          acc[e] = first ? g : add2(acc[e], g);
+        }
+      }
+      if ((u + 1) % a.share == 0) {
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(b_empty + (jt & 1));
+        if (i < a.nq) {
+          Bf *dst = static_cast<Bf *>(p.x.dbias) + ((int64_t(bb) * a.heads + h) * a.nq + i) * p.x.dbias_ld;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(lo_f(acc[4 * c + e]), hi_f(acc[4 * c + e]));
+            const int k = k0 + 8 * c;
+            if (k + 8 <= a.nk)
+              *reinterpret_cast<uint4 *>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            else
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (k + e < a.nk) reinterpret_cast<uint16_t *>(dst)[k + e] = uint16_t(w[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 128);
+  }
+}
+
+// The six maps of a kernel whose resident tiles are 128 rows; false where TMA cannot describe one.
+bool back_maps(CUtensorMap (&m)[6], const BackArgs &x, bool queries_resident) {
+  const Args &a = x.a;
+  const int kv_heads = a.heads / a.group, qr = queries_resident ? kRowsTc : kTileTc, kr = queries_resident ? kTileTc : kRowsTc;
+  const Rows dout{x.dout, int64_t(a.nq) * a.heads * a.d, int64_t(a.heads) * a.d, a.d};
+  Rows low = dout;
+  if (x.dlow) low.p = x.dlow;
+  if (!rows_map(&m[0], a.q, a.d, a.nq, a.heads, a.batch, qr) || !rows_map(&m[1], dout, a.d, a.nq, a.heads, a.batch, qr) ||
+      !rows_map(&m[2], low, a.d, a.nq, a.heads, a.batch, qr) || !rows_map(&m[3], a.k, a.d, a.nk, kv_heads, a.batch, kr) ||
+      !rows_map(&m[4], a.v, a.d, a.nk, kv_heads, a.batch, kr))
+    return false;
+  m[5] = m[0];
+  const Rows bias{a.bias, a.bias_sb, a.bias_si, a.bias_sh};
+  return !a.bias || rows_map(&m[5], bias, a.nk, a.nq, a.heads, a.batch / a.share, qr);
+}
+
+bool back_covered(const Args &a) {
+  return a.nk >= 64 && a.nq >= 64 && !(a.bias && !a.bias_vec) && a.batch > 0;
+}
+
+template <typename K> int back_launch(K kernel, int bytes, const BackTc &p, int64_t ctas, const CUtensorMap (&m)[6], cudaStream_t stream) {
+  BL_REQUIRE(p.status, "bl_cross_attention_backward: device status word unavailable");
+  BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention_backward: too many tiles");
+  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(kernel), bytes));
+  kernel<<<unsigned(ctas), kThreadsTc, bytes, stream>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+  BL_LAUNCH_CHECK();
+  return BL_OK;
+}
+
+}  // namespace
+
+#define BL_PICK(KERNEL, SHAPE, W, B, L)                                                                       \
+  do {                                                                                                        \
+    static_assert(SHAPE<W, B, L>::kBytes <= 232448, "shared memory");                                         \
+    return back_launch(KERNEL<W, B, L>, SHAPE<W, B, L>::kBytes, p, ctas, maps, stream);                       \
+  } while (0)
+#define BL_DISPATCH(KERNEL, SHAPE)                                                                            \
+  do {                                                                                                        \
+    if (a.d > 64) {                                                                                           \
+      if (a.bias) { if (x.dlow) BL_PICK(KERNEL, SHAPE, 2, true, true); BL_PICK(KERNEL, SHAPE, 2, true, false); } \
+      if (x.dlow) BL_PICK(KERNEL, SHAPE, 2, false, true);                                                     \
+      BL_PICK(KERNEL, SHAPE, 2, false, false);                                                                \
+    }                                                                                                         \
+    if (a.bias) { if (x.dlow) BL_PICK(KERNEL, SHAPE, 1, true, true); BL_PICK(KERNEL, SHAPE, 1, true, false); } \
+    if (x.dlow) BL_PICK(KERNEL, SHAPE, 1, false, true);                                                       \
+    BL_PICK(KERNEL, SHAPE, 1, false, false);                                                                  \
+  } while (0)
+
+int queries_tc(const BackArgs &x, cudaStream_t stream, bool *taken) {
+  const Args &a = x.a;
+  CUtensorMap maps[6];
+  *taken = back_covered(a) && back_maps(maps, x, true);
+  if (!*taken) return BL_OK;
+  BackTc p{x, (a.nq + kRowsTc - 1) / kRowsTc, device_status_ptr()};
+  const int64_t ctas = int64_t(p.tiles) * a.heads * a.batch;
+  BL_DISPATCH(queries_tc_kernel, QShape);
+}
+
+int keys_tc(const BackArgs &x, cudaStream_t stream, bool *taken) {
+  const Args &a = x.a;
+  CUtensorMap maps[6];
+  *taken = back_covered(a) && back_maps(maps, x, false);
+  if (!*taken) return BL_OK;
+  BackTc p{x, (a.nk + kRowsTc - 1) / kRowsTc, device_status_ptr()};
+  const int64_t ctas = int64_t(p.tiles) * (a.heads / a.group) * a.batch;
+  BL_DISPATCH(keys_tc_kernel, KShape);
+}
+
+int bias_tc(const BackArgs &x, cudaStream_t stream, bool *taken) {
+  const Args &a = x.a;
+  CUtensorMap maps[6];
+  *taken = a.d <= 64 && back_covered(a) && back_maps(maps, x, true);
+  if (!*taken) return BL_OK;
+  BackTc p{x, (a.nq + kRowsTc - 1) / kRowsTc, device_status_ptr()};
+  BL_REQUIRE(p.status, "bl_cross_attention_backward: device status word unavailable");
+  // Few row tiles: the keys are divided so that one wave of CTAs (one per SM) covers them.
+  const int64_t base = int64_t(p.tiles) * a.heads * (a.batch / a.share), key_tiles = (a.nk + kTileTc - 1) / kTileTc;
+  int64_t ranges = num_sms() / base;
+  ranges = ranges < 1 ? 1 : ranges > key_tiles ? key_tiles : ranges;
+  BL_REQUIRE(base * ranges < (int64_t(1) << 31), "bl_cross_attention_backward: too many bias blocks");
+  auto kernel = x.dlow ? bias_tc_kernel<true> : bias_tc_kernel<false>;
+  const int bytes = x.dlow ? BShape<true>::kBytes : BShape<false>::kBytes;
+  static_assert(BShape<true>::kBytes <= 232448, "shared memory");
+  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(kernel), bytes));
+  kernel<<<unsigned(base * ranges), kThreadsTc, bytes, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p,
+                                                                 int(ranges));
+  BL_LAUNCH_CHECK();
+  return BL_OK;
+}
+
+}  // namespace xa
+}  // namespace bl
