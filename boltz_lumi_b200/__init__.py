@@ -8,6 +8,8 @@ Drop-in for the module API of upstream Boltz 2.2.1:
   ConditionedTransitionBlock);
 * :mod:`boltz_lumi_b200.layers` holds standalone modules with the upstream
   constructors and parameter names;
+* :mod:`boltz_lumi_b200.autograd` holds the operators that also train (relative
+  position encoding and bias, cross attention);
 * ``python -m boltz_lumi_b200 predict ...`` wraps the Boltz CLI.
 
 All compute runs in ``libboltz_b200.so`` (C ABI: ``include/boltz_b200.h``).

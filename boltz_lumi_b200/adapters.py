@@ -95,7 +95,8 @@ def _token_attention(self, s, z, mask, k_in, multiplicity=1):
     if (not _inference(self, s, z, mask, k_in) or self.compute_pair_bias or torch.is_autocast_enabled("cuda")):
         return cls.forward(self, s, z, mask, k_in, multiplicity)
     bias = self.proj_z(z)
-    if (not forwards.token_attention_supported(self, s, k_in, bias, mask)
+    supported = (forwards.token_attention_supported if k_in.shape == s.shape else forwards.cross_attention_supported)
+    if (not supported(self, s, k_in, bias, mask)
             or bias.shape[0] * multiplicity not in (s.shape[0], 1)):
         return cls.forward(self, s, z, mask, k_in, multiplicity)
     return forwards.attend_with_bias(self, s, bias, mask, k_in)
@@ -140,7 +141,11 @@ def _graphed_score_model(structure):
         step.reset()
 
 
-def install(model, require_device=True, cuda_graphs=False):
+_ATOM_TRANSFORMERS = ("structure_module.score_model.atom_attention_encoder.",
+                      "structure_module.score_model.atom_attention_decoder.")
+
+
+def install(model, require_device=True, cuda_graphs=False, atom_attention=False):
     """Rebind the hot-path forwards of ``model`` in place; idempotent.
 
     Returns the number of modules rebound.  Like the reference, modules are
@@ -153,7 +158,10 @@ def install(model, require_device=True, cuda_graphs=False):
     bias is packed once per prediction.  ``cuda_graphs=True`` additionally
     replays the score model of each sampling call from a CUDA graph
     (:mod:`boltz_lumi_b200.graphs`); it needs a capture-safe score model and is
-    off by default.
+    off by default.  ``atom_attention=True`` also rebinds the AttentionPairBias
+    modules of the atom encoder and decoder (windows of 32 queries to 128 keys,
+    :func:`forwards.cross_attend_with_bias`), which the reference leaves to
+    upstream's eager code; off by default.
     """
     if getattr(model, "_b200_optimized", False):
         return 0
@@ -174,7 +182,9 @@ def install(model, require_device=True, cuda_graphs=False):
         elif cls in _DIFFUSION and name.startswith("structure_module.score_model."):
             module.forward = MethodType(_adaln if cls == "AdaLN" else _conditioned_transition, module)
             count += 1
-        elif cls == "AttentionPairBias" and name.startswith("structure_module.score_model.token_transformer."):
+        elif cls == "AttentionPairBias" and (
+                name.startswith("structure_module.score_model.token_transformer.")
+                or atom_attention and name.startswith(_ATOM_TRANSFORMERS)):
             module.forward = MethodType(_token_attention, module)
             count += 1
     structure = getattr(model, "structure_module", None)

@@ -506,6 +506,43 @@ def token_attention_supported(module, s, k_in, bias, mask=None):
             and all(p.bias is None for p in (module.proj_k, module.proj_v, module.proj_g)))
 
 
+def cross_attention_supported(module, s, k_in, bias, mask=None):
+    """Shapes and dtypes the fp32 attention of ``s`` [B, Nq, c] to states ``k_in`` [B, Nk, c] of another length covers."""
+    heads, d = module.num_heads, module.head_dim
+    return (d % 8 == 0 and 8 <= d <= 128 and heads * d == module.c_s and s.dim() == 3 and k_in.dim() == 3
+            and s.dtype == k_in.dtype == torch.float32 and s.is_cuda and k_in.is_cuda
+            and s.shape[0] == k_in.shape[0] and s.shape[-1] == k_in.shape[-1] == module.c_s
+            and bias.dim() == 4 and tuple(bias.shape[1:]) == (heads, s.shape[1], k_in.shape[1])
+            and bias.shape[0] >= 1 and s.shape[0] % bias.shape[0] == 0 and bias.device == s.device
+            and (mask is None or tuple(mask.shape) == tuple(k_in.shape[:2]))
+            and all(p.bias is None for p in (module.proj_k, module.proj_v, module.proj_g)))
+
+
+def cross_attend_with_bias(self, s, bias, mask, k_in, residual=None):
+    """:func:`attend_with_bias` for ``k_in`` of another length than ``s``: the atom transformer's windows (32 queries
+    to 128 keys), or tokens attending to atoms.  ``bias`` [B', H, Nq, Nk], ``mask`` [B, Nk] over the keys.  q | g and
+    k | v are one GEMM each; :func:`kernels.cross_attention` reads the column blocks in place."""
+    if not cross_attention_supported(self, s, k_in, bias, mask):
+        raise RuntimeError(f"cross attention covers fp32 CUDA s [B, Nq, H*d] and k_in [B, Nk, H*d] with d % 8 == 0, "
+                           f"d <= 128, bias [B', H, Nq, Nk] and mask [B, Nk]; got s {tuple(s.shape)}, "
+                           f"k_in {tuple(k_in.shape)}, bias {tuple(bias.shape)}")
+    heads, d = self.num_heads, self.head_dim
+    with torch.autocast("cuda", enabled=False):  # the reference's math is fp32 throughout
+        qg = _linear32(self, "_bl_w3_qg", s, [self.proj_q.weight, self.proj_g.weight], [self.proj_q.bias, None])
+        kv = _linear32(self, "_bl_w3_kv", k_in, [self.proj_k.weight, self.proj_v.weight])
+        q, g = (t.unflatten(-1, (heads, d)) for t in qg.chunk(2, -1))
+        k, v = (t.unflatten(-1, (heads, d)) for t in kv.chunk(2, -1))
+        inf = None if mask is None else self.inf
+        o = kernels.cross_attention(q, k, v, bias=bias.float(), mask=mask, inf=inf, gate=g,
+                                    scale=kernels.attention_scale(d))
+        o = o.flatten(2)
+        if o.shape[-1] % 8 == 0 and o.numel():
+            return _linear32_planes(self, "_bl_w3_o", kernels.split3_fast(o), o.shape[:2], [self.proj_o.weight],
+                                    [self.proj_o.bias], residual=residual)
+        y = F.linear(o, self.proj_o.weight, self.proj_o.bias)
+        return y if residual is None else y + residual
+
+
 def attend_with_bias(self, s, bias, mask, k_in, s3=None, residual=None):
     """Upstream attentionv2 ``AttentionPairBias`` after ``proj_z``: projections,
     fused fp32 attention with bias, key mask and sigmoid gate, then ``proj_o``.
@@ -517,6 +554,8 @@ def attend_with_bias(self, s, bias, mask, k_in, s3=None, residual=None):
     giving the shape.  With ``residual`` the result is ``residual + attention``
     (the add runs in proj_o's epilogue).
     """
+    if k_in.dim() == 3 and s.dim() == 3 and k_in.shape[1] != s.shape[1]:
+        return cross_attend_with_bias(self, s, bias, mask, k_in, residual=residual)
     if not token_attention_supported(self, s, k_in, bias, mask):
         raise RuntimeError(f"token attention covers fp32 CUDA s [B, N, H*d] with d in {_TOKEN_HEAD_DIMS}, "
                            f"bias [B', H, N, N] and mask [B, N]; got s {tuple(s.shape)}, bias {tuple(bias.shape)}")
@@ -587,6 +626,7 @@ def normalization_forward(self, x):
 __all__ = [
     "adaln_forward",
     "attend_with_bias",
+    "cross_attend_with_bias",
     "prepare_token_bias",
     "token_attention_forward",
     "conditioned_transition_forward",

@@ -11,7 +11,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _lib, forwards, kernels
+from . import _lib, autograd, forwards, kernels
 
 
 def _inference_only(module):
@@ -144,7 +144,9 @@ class AttentionPairBias(nn.Module):
 
     With ``compute_pair_bias`` the bias is LayerNorm(z) . W_z (the Pairformer
     block); without it ``z`` is the bias itself, [B, N, N, H] (the diffusion
-    token transformer's layer slice of the prepared token bias).
+    token transformer's layer slice of the prepared token bias).  ``k_in`` may be
+    of another length than ``s`` (the atom transformer's windows: z [B, Nq, Nk, H],
+    mask over the keys).
     """
 
     def __init__(self, c_s, c_z=None, num_heads=None, inf=1e6, compute_pair_bias=True):
@@ -184,6 +186,39 @@ class AttentionPairBias(nn.Module):
         """The attention given the pair bias [b', heads, N, N] (fp32, b' dividing b), plus
         ``residual`` when given (added in proj_o's epilogue)."""
         return forwards.attend_with_bias(self, s, bias, mask, k_in, residual=residual)
+
+
+class RelativePositionEncoder(nn.Module):
+    """Relative position encoding of token pairs (upstream's constructor and ``linear_layer`` weight; AF3 supplementary
+    Algorithm 3).  Unlike the other modules it also trains: with grad mode on, gradients of the weight are recorded.
+
+    ``forward(feats)`` takes upstream's feature dict (``residue_index``, ``asym_id``, ``entity_id``, ``token_index``,
+    ``sym_id``, integers [B, N]) and returns [B, N, N, token_z], bf16 under bf16 autocast and fp32 otherwise.
+    ``add_to(z, feats)`` adds the encoding into a contiguous fp32 pair tensor in place (inference).  Upstream's cyclic
+    chains (``cyclic_pos_enc``) are not covered.
+    """
+
+    def __init__(self, token_z, r_max=32, s_max=2, fix_sym_check=False, cyclic_pos_enc=False):
+        super().__init__()
+        if cyclic_pos_enc:
+            raise NotImplementedError("RelativePositionEncoder does not cover cyclic chains")
+        self.r_max, self.s_max, self.fix_sym_check = r_max, s_max, fix_sym_check
+        self.linear_layer = nn.Linear(kernels.relative_position_columns(r_max, s_max), token_z, bias=False)
+
+    @staticmethod
+    def _features(feats):
+        return [feats[k] for k in ("residue_index", "asym_id", "entity_id", "token_index", "sym_id")]
+
+    def forward(self, feats):
+        short = torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
+        return autograd.relative_position_encoding(
+            self.linear_layer.weight, *self._features(feats), self.r_max, self.s_max, self.fix_sym_check,
+            torch.bfloat16 if short else torch.float32)
+
+    def add_to(self, z, feats):
+        _inference_only(self)
+        return kernels.relative_position_encoding(self.linear_layer.weight, *self._features(feats), self.r_max,
+                                                  self.s_max, self.fix_sym_check, residual=z)
 
 
 class _FP32Transition(Transition):

@@ -102,3 +102,38 @@ def test_arguments_filled(monkeypatch):
     turned = torch.zeros(1, 4, 5, 3).transpose(2, 3)  # a bias without contiguous rows is laid out in padded rows
     x, (_, _, _, b, _, _) = shaped(bias=turned)
     assert list(x.bias_stride) == [4 * 3 * 8, 3 * 8, 8]
+
+
+def test_install_rebinds_atom_attention_on_request():
+    from torch import nn
+
+    from boltz_lumi_b200 import adapters, layers
+
+    model = nn.Module()
+    model.structure_module = nn.Module()
+    score = model.structure_module.score_model = nn.Module()
+    for name in ("atom_attention_encoder", "atom_attention_decoder", "token_transformer"):
+        part = nn.Module()
+        part.attention = layers.AttentionPairBias(64, num_heads=4, compute_pair_bias=False)
+        setattr(score, name, part)
+    assert adapters.install(model, require_device=False) == 1
+    adapters.uninstall(model)
+    assert adapters.install(model, require_device=False, atom_attention=True) == 3
+    assert "forward" in score.atom_attention_decoder.attention.__dict__
+    adapters.uninstall(model)
+    assert "forward" not in score.atom_attention_decoder.attention.__dict__
+
+
+def test_cross_lengths_refused_on_cpu():
+    from boltz_lumi_b200 import forwards, layers
+
+    m = layers.AttentionPairBias(64, num_heads=4, compute_pair_bias=False).eval()
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="cross attention covers"):
+        forwards.attend_with_bias(m, torch.zeros(1, 3, 64), torch.zeros(1, 4, 3, 5), torch.ones(1, 5), torch.zeros(1, 5, 64))
+
+
+def test_relative_position_encoder_refuses_cyclic():
+    from boltz_lumi_b200 import layers
+
+    with pytest.raises(NotImplementedError, match="cyclic"):
+        layers.RelativePositionEncoder(128, cyclic_pos_enc=True)
