@@ -4,6 +4,8 @@
 // warp; key tiles of kBN stream through a two-stage cp.async ring (K, V, the
 // bias block) while the previous tile is computed; running maximum and sum in
 // fp32 registers; the [Nq, Nk] scores never exist in memory.
+#include <array>
+
 #include "cross_attention.cuh"
 
 namespace bl {
@@ -194,16 +196,19 @@ template <typename T, int DP> int launch_flash(const Args &a, cudaStream_t strea
 // and output.  The warps' parts are merged in shared memory, the CTAs' parts
 // through distributed shared memory: one launch, no workspace, fixed order.
 // ---------------------------------------------------------------------------
-constexpr int kStepWarps = 4, kStepStages = 3, kStepRows = 16;
+constexpr int kStepRows = 16;
 
 template <typename T, int DP> struct Step {
+  // Eight warps (two per scheduler: a chunk is a chain of some 600 instructions) with two
+  // chunks each in flight; wide rows leave room for four warps with three.
+  static constexpr int warps = DP == 128 ? 4 : 8, stages = DP == 128 ? 3 : 2;
   static constexpr int kc = (sizeof(T) == 4 && DP >= 64) ? 16 : 32, ld = kLd<T, DP>;
   static constexpr int kv = kc * ld;              // elements of a K or V chunk
   static constexpr int bias = kStepRows * (kc + 8);
   static constexpr int stage_bytes = (2 * kv + bias) * int(sizeof(T)) + kc * 4;
   static constexpr int q_bytes = kStepRows * ld * int(sizeof(T));
-  static constexpr int ring_bytes = kStepWarps * kStepStages * stage_bytes;
-  static constexpr int part_bytes = (kStepWarps * kStepRows * (DP + 2) + 2 * kStepRows) * 4;
+  static constexpr int ring_bytes = warps * stages * stage_bytes;
+  static constexpr int part_bytes = (warps * kStepRows * (DP + 2) + 2 * kStepRows) * 4;
   static constexpr int bytes = q_bytes + (ring_bytes > part_bytes ? ring_bytes : part_bytes);
 };
 
@@ -219,8 +224,9 @@ __device__ __forceinline__ float peer(const float *local, uint32_t rank) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, int split) {
+__global__ void __launch_bounds__(32 * Step<T, DP>::warps) step_kernel(const Args a, int split) {
   using S = Step<T, DP>;
+  constexpr int kStepWarps = S::warps, kStepStages = S::stages;
   constexpr int KC = S::kc, NT = KC / 8, ld = S::ld, ND = DP / 8, kVec = Type<T>::kVec, kChunks = DP / kVec;
   extern __shared__ float4 smem4[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -252,14 +258,17 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, int
       float *mk = reinterpret_cast<float *>(bt + S::bias);
       const int j0 = next * KC;
       if (lane < KC) mk[lane] = mk_next;
+      // Lane: chunk c of rows r0, r0 + kStep, ...
+      constexpr int kStep = 32 / kChunks > 0 ? 32 / kChunks : 1;
+      const int r0 = lane / kChunks, c = lane % kChunks * kVec;
+      const uint32_t gone = __ballot_sync(0xffffffffu, mk_next == -INFINITY);
+      const T *kp = k + int64_t(j0 + r0) * a.k.si + c, *vp = v + int64_t(j0 + r0) * a.v.si + c;
+      const int64_t k_step = kStep * a.k.si, v_step = kStep * a.v.si;
 #pragma unroll 4
-      for (int u = lane; u < KC * kChunks; u += 32) {
-        const int r = u / kChunks, c = u % kChunks * kVec;
-        const float m = __shfl_sync(0xffffffffu, mk_next, r);
-        const bool ok = m != -INFINITY && c < a.d;
-        const int64_t j = ok ? j0 + r : 0;
-        cp16(kt + r * ld + c, k + (ok ? j * a.k.si + c : 0), ok ? 16 : 0);
-        cp16(vt + r * ld + c, v + (ok ? j * a.v.si + c : 0), ok ? 16 : 0);
+      for (int r = r0; r < KC; r += kStep, kp += k_step, vp += v_step) {
+        const bool ok = (gone >> r & 1) == 0 && c < a.d;
+        cp16(kt + r * ld + c, ok ? kp : k, ok ? 16 : 0);
+        cp16(vt + r * ld + c, ok ? vp : v, ok ? 16 : 0);
       }
       if (bias) {
         for (int u = lane; u < rows * (KC / kVec); u += 32) {
@@ -336,8 +345,9 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, int
             sum += s[n][2 * r + e];
           }
         l[r] = fmaf(l[r], alpha, sum);
+        if (__any_sync(0xffffffffu, alpha != 1.f))
 #pragma unroll
-        for (int n = 0; n < ND; ++n) o[n][2 * r] *= alpha, o[n][2 * r + 1] *= alpha;
+          for (int n = 0; n < ND; ++n) o[n][2 * r] *= alpha, o[n][2 * r + 1] *= alpha;
       }
       mma_acc<NT, DP>(o, s, vt, lane);
     }
@@ -415,17 +425,48 @@ __global__ void __launch_bounds__(32 * kStepWarps) step_kernel(const Args a, int
   if (split > 1) cluster_barrier();  // peers may still be reading this CTA's parts
 }
 
+// Clusters of s CTAs that the device holds at once (1 / s of its SMs where the query fails).
+template <typename T, int DP> int active_clusters(int s) {
+  using S = Step<T, DP>;
+  static const std::array<int, 9> table = [] {
+    std::array<int, 9> t{};
+    for (int e = 1; e <= 8; ++e) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = unsigned(e), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(unsigned(e)), config.blockDim = dim3(32 * S::warps), config.dynamicSmemBytes = S::bytes;
+      config.attrs = attr, config.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, step_kernel<T, DP>, &config) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = num_sms() / e;
+      }
+      t[e] = n < 1 ? 1 : n;
+    }
+    return t;
+  }();
+  return table[s];
+}
+
 template <typename T, int DP> int launch_step(const Args &a, cudaStream_t stream) {
   using S = Step<T, DP>;
+  static_assert(S::bytes <= 232448, "shared memory");
   const int64_t slabs = int64_t(a.batch) * (a.heads / a.group);
-  // Enough CTAs for every SM, with at least two chunks per warp.
-  int split = 1;
-  while (split < 8 && slabs * split < num_sms() && a.nk >= 4 * split * kStepWarps * S::kc) split *= 2;
-  BL_REQUIRE(slabs * split < (int64_t(1) << 31), "bl_cross_attention: too many samples");
   BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(step_kernel<T, DP>), S::bytes));
+  // The split with the fewest waves per CTA's share of the keys, at least one chunk per warp.  (A fixed split of
+  // eight took two waves at 20 slabs: 62 us against 31.)
+  int split = 1;
+  double best = 0.;
+  for (int e = 1; e <= 8 && (e == 1 || a.nk >= int64_t(e) * S::warps * S::kc); ++e) {
+    const int64_t waves = (slabs + active_clusters<T, DP>(e) - 1) / active_clusters<T, DP>(e);
+    const double cost = double(waves) / e + 0.02 * (e > 1);  // a cluster's merge costs a little
+    if (e == 1 || cost < best) best = cost, split = e;
+  }
+  BL_REQUIRE(slabs * split < (int64_t(1) << 31), "bl_cross_attention: too many samples");
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(slabs * split));
-  config.blockDim = dim3(32 * kStepWarps);
+  config.blockDim = dim3(32 * S::warps);
   config.dynamicSmemBytes = S::bytes;
   config.stream = stream;
   cudaLaunchAttribute attr[1];
