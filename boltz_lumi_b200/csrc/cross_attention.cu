@@ -12,7 +12,7 @@ namespace bl {
 namespace xa {
 namespace {
 
-template <typename T, int DP> constexpr int kBN = (sizeof(T) == 4 && DP == 128) ? 32 : 64;
+template <typename T, int DP> constexpr int kBN = sizeof(T) == 4 ? 32 : 64;
 
 template <typename T, int DP> struct FlashSmem {
   static constexpr int bn = kBN<T, DP>, ld = kLd<T, DP>;

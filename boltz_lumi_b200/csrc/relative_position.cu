@@ -39,14 +39,21 @@ __device__ __forceinline__ uint32_t clip_offset(int64_t a, int64_t b, int m) {
   const int64_t d = a - b;
   return uint32_t(d < -m ? 0 : d > m ? 2 * m : int(d) + m);
 }
-__device__ __forceinline__ uint32_t pick(const EncArgs &a, int64_t i, int64_t j) {
-  const int64_t ri = a.residue[i], rj = a.residue[j];
-  const bool chain = a.asym[i] == a.asym[j], agree = a.entity[i] == a.entity[j];
+// The features of a pair as loaded: looked at only later, so that the loads stay in flight.
+struct PairFeatures {
+  int64_t ri, rj, ai, aj, ei, ej, ti, tj, si, sj;
+};
+__device__ __forceinline__ PairFeatures pair_features(const EncArgs &a, int64_t i, int64_t j) {
+  return {a.residue[i], a.residue[j], a.asym[i],  a.asym[j], a.entity[i],
+          a.entity[j],  a.token[i],   a.token[j], a.sym[i],  a.sym[j]};
+}
+__device__ __forceinline__ uint32_t pick(const EncArgs &a, const PairFeatures &f) {
+  const bool chain = f.ai == f.aj, agree = f.ei == f.ej;
   const uint32_t apart = 2 * a.r + 1;
-  const uint32_t p = chain ? clip_offset(ri, rj, a.r) : apart;
-  const uint32_t t = apart + 1 + (chain && ri == rj ? clip_offset(a.token[i], a.token[j], a.r) : apart);
+  const uint32_t p = chain ? clip_offset(f.ri, f.rj, a.r) : apart;
+  const uint32_t t = apart + 1 + (chain && f.ri == f.rj ? clip_offset(f.ti, f.tj, a.r) : apart);
   const bool other = a.fix_sym ? !agree : chain;
-  const uint32_t c = 2 * (apart + 1) + 1 + (other ? 2 * a.s + 1 : clip_offset(a.sym[i], a.sym[j], a.s));
+  const uint32_t c = 2 * (apart + 1) + 1 + (other ? 2 * a.s + 1 : clip_offset(f.si, f.sj, a.s));
   return p | (t << 10) | (c << 20) | (uint32_t(agree) << 30);
 }
 
@@ -76,13 +83,18 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
+__device__ __forceinline__ void put4(float *p, float4 y) { *reinterpret_cast<float4 *>(p) = y; }
+__device__ __forceinline__ void put4(__nv_bfloat16 *p, float4 y) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+}
+
 // kLanes lanes (4 channels each) per pair; a warp step writes 32 / kLanes
 // pairs.  A warp takes 32 consecutive pairs of one row i: lane l computes the
 // picks of pair j0 + l, the others receive them by shuffle.  The sum of the
 // token, entity and chain rows repeats along most of a row, so it stays in
-// registers until its picks change: one shared load per pair and lane.
+// registers: one shared load per pair and lane.
 template <typename Out, int kLanes, bool kAdd>
-__global__ void __launch_bounds__(256) encoding_kernel(const float *w, const EncArgs a, Out *out) {
+__global__ void __launch_bounds__(1024) encoding_kernel(const float *w, const EncArgs a, Out *out) {
   constexpr int kC = 4 * kLanes, kLd = kC + 4, kPairs = 32 / kLanes;
   extern __shared__ float4 smem4[];
   float *rows = reinterpret_cast<float *>(smem4);
@@ -97,114 +109,144 @@ __global__ void __launch_bounds__(256) encoding_kernel(const float *w, const Enc
   const float *col = rows + c;
   uint32_t held = 0xffffffffu;
   float4 base = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto hold = [&](uint32_t key) {
+    held = key;
+    base = add4(*reinterpret_cast<const float4 *>(col + (key & 1023u) * kLd),
+                *reinterpret_cast<const float4 *>(col + ((key >> 10) & 1023u) * kLd));
+    if (key >> 20) base = add4(base, *reinterpret_cast<const float4 *>(col + (4 * a.r + 4) * kLd));
+  };
+  auto write = [&](Out *p, uint32_t row) {
+    float4 y = add4(*reinterpret_cast<const float4 *>(col + row * kLd), base);
+    if constexpr (kAdd) y = add4(y, *reinterpret_cast<const float4 *>(p));
+    put4(p, y);
+  };
   for (uint32_t u = blockIdx.x * warps + (threadIdx.x >> 5); u < units; u += gridDim.x * warps) {
     const uint32_t row = u / uint32_t(segments);  // b * n + i
     const int j0 = int(u - row * segments) * 32;
     const int64_t i = row, b0 = row / uint32_t(n) * n;
-    const uint32_t mine = j0 + lane < n ? pick(a, i, b0 + j0 + lane) : 0u;
     const int count = n - j0 < 32 ? n - j0 : 32;
-    Out *dst = out + (i * n + j0) * a.channels + c0 + c;
-#pragma unroll 4
-    for (int t = 0; t < count; t += kPairs) {
-      const int jj = t + sub;
-      const uint32_t v = __shfl_sync(0xffffffffu, mine, jj & 31);
-      if (jj < count && live) {
-        if ((v >> 10) != held) {
-          held = v >> 10;
-          base = add4(*reinterpret_cast<const float4 *>(col + ((v >> 10) & 1023u) * kLd),
-                      *reinterpret_cast<const float4 *>(col + ((v >> 20) & 1023u) * kLd));
-          if (v >> 30) base = add4(base, *reinterpret_cast<const float4 *>(col + (4 * a.r + 4) * kLd));
-        }
-        float4 y = add4(*reinterpret_cast<const float4 *>(col + (v & 1023u) * kLd), base);
-        Out *p = dst + int64_t(jj) * a.channels;
-        if constexpr (sizeof(Out) == 4) {
-          if (kAdd) y = add4(y, *reinterpret_cast<const float4 *>(p));
-          *reinterpret_cast<float4 *>(p) = y;
-        } else {
-          *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+    uint32_t mine = 0;
+    if (lane < count) mine = pick(a, pair_features(a, i, b0 + j0 + lane));
+    const uint32_t key = __shfl_sync(0xffffffffu, mine, 0) >> 10;
+    Out *p = out + (i * n + j0 + sub) * a.channels + c0 + c;
+    const int64_t step = int64_t(kPairs) * a.channels;
+    if (count == 32 && __all_sync(0xffffffffu, (mine >> 10) == key)) {
+      // One base for the whole segment.
+      if (key != held) hold(key);
+#pragma unroll 8
+      for (int t = 0; t < 32; t += kPairs, p += step) {
+        const uint32_t v = __shfl_sync(0xffffffffu, mine, t + sub) & 1023u;
+        if (kLanes == 32 || live) write(p, v);
+      }
+    } else {
+      for (int t = 0; t < count; t += kPairs, p += step) {
+        const uint32_t v = __shfl_sync(0xffffffffu, mine, (t + sub) & 31);
+        if (t + sub < count && live) {
+          if ((v >> 10) != held) hold(v >> 10);
+          write(p, v & 1023u);
         }
       }
     }
   }
 }
 
-// Gradient of W.  A group of two warps covers 128 channels (two per lane) and owns
-// a private [rows][128] table in shared memory, each element of which one lane
-// alone updates.  A group walks diagonals: from pair (i0, j) it visits
-// (i0 + s, (j + s) mod n) for up to kSteps rows, every load a coalesced half of a
-// pair row, all of a walk's loads in flight at once.  Along a diagonal of one chain
-// the offsets, so the picks, do not change: the sum of the pairs stays in registers
-// and goes to the table rows of its picks when one of them changes.
+// Gradient of W.  A warp covers 128 channels (four per lane) and owns a private
+// [rows][128] table in shared memory, each element of which one lane alone
+// updates.  It walks diagonals: from pair (i0, j) it visits (i0 + s, (j + s) mod n)
+// for up to kSteps rows, every load a whole pair row, two walks' loads in flight at
+// once.  Along a diagonal of one chain the offsets, so the picks, do not change: the
+// sum of the pairs stays in registers and goes to the table rows of its picks when one
+// of them changes.
 constexpr int kGroups = 3;  // private tables per CTA (71 KB each at r = 32, s = 2)
-template <typename In> constexpr int kSteps = sizeof(In) == 4 ? 32 : 64;
+template <typename In> constexpr int kSteps = sizeof(In) == 4 ? 16 : 32;
+
+__device__ __forceinline__ float4 as_float4(float4 v) { return v; }
+__device__ __forceinline__ float4 as_float4(uint2 v) {
+  return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+}
 
 template <typename In>
-__global__ void __launch_bounds__(kGroups * 64) encoding_grad_kernel(const In *grad, const EncArgs a, float *partial) {
+__global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *grad, const EncArgs a, float *partial) {
   constexpr int kS = kSteps<In>;
+  using Raw = typename std::conditional<sizeof(In) == 4, float4, uint2>::type;
   extern __shared__ float4 smem4[];
   float *tables = reinterpret_cast<float *>(smem4);
-  const int groups = blockDim.x / 64, size = a.rows * 128;
+  const int groups = blockDim.x / 32, size = a.rows * 128;
   for (int i = threadIdx.x; i < groups * size / 4; i += blockDim.x) smem4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  const int lane = threadIdx.x & 31, group = threadIdx.x / 64;
-  const int ch = threadIdx.x % 64 * 2, c0 = blockIdx.y * 128;
-  const bool live = c0 + ch < a.channels;  // channels is even
-  float2 *mine = reinterpret_cast<float2 *>(tables + group * size + ch);
+  const int lane = threadIdx.x & 31, group = threadIdx.x / 32, ch = 4 * lane, c0 = blockIdx.y * 128;
+  const bool live = c0 + ch < a.channels;  // channels is a multiple of 4
+  float4 *mine = reinterpret_cast<float4 *>(tables + group * size + ch);
   const int n = a.n, blocks = (n + kS - 1) / kS;
   const uint32_t units = uint32_t(a.batch * blocks * n);
   const int64_t step = (int64_t(n) + 1) * a.channels, wrap = int64_t(n) * a.channels;
-  float2 run = make_float2(0.f, 0.f);
+  float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
   uint32_t held = 0xffffffffu;
-  auto put = [&](uint32_t row) {
-    float2 v = mine[row * 64];
-    v.x += run.x, v.y += run.y;
-    mine[row * 64] = v;
-  };
+  auto put = [&](uint32_t row) { mine[row * 32] = add4(mine[row * 32], run); };
   auto flush = [&]() {
     put(held & 1023u), put((held >> 10) & 1023u), put((held >> 20) & 1023u);
     if (held >> 30) put(4 * a.r + 4);
-    run = make_float2(0.f, 0.f);
+    run = make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  for (uint32_t u = blockIdx.x * groups + group; u < units; u += gridDim.x * groups) {
+  struct Walk {
+    Raw x[kS];
+    PairFeatures f;  // of step `lane`
+    int count;
+  };
+  auto load = [&](uint32_t u, Walk &w) {
     const uint32_t ib = u / uint32_t(n), b = ib / uint32_t(blocks);
     const int j = int(u - ib * n), i0 = int(ib - b * blocks) * kS;
     const int64_t b0 = int64_t(b) * n;
-    const int count = n - i0 < kS ? n - i0 : kS;
+    w.count = u >= units ? 0 : n - i0 < kS ? n - i0 : kS;
     const In *p = grad + ((b0 + i0) * n + j) * a.channels + c0 + ch;
-    typename std::conditional<sizeof(In) == 4, float2, uint32_t>::type x[kS];
-    int col = j;
+    const int turn = n - j;  // first step past the row's end (s < count <= n: at most one turn)
+    const int last = live ? w.count : 0;
 #pragma unroll
     for (int s = 0; s < kS; ++s) {
-      if (s < count && live) {
-        if constexpr (sizeof(In) == 4)
-          x[s] = __ldcs(reinterpret_cast<const float2 *>(p));
-        else
-          x[s] = __ldcs(reinterpret_cast<const unsigned int *>(p));
-      } else {
-        x[s] = {};
-      }
+      if (s == turn) p -= wrap;
+      w.x[s] = {};
+      if (s < last) w.x[s] = __ldcs(reinterpret_cast<const Raw *>(p));
       p += step;
-      if (++col == n) col = 0, p -= wrap;
     }
-    uint32_t packed[kS / 32];
-#pragma unroll
-    for (int e = 0; e < kS / 32; ++e) {
-      const int s = 32 * e + lane;
-      packed[e] = s < count ? pick(a, b0 + i0 + s, b0 + (j + s) % n) : 0u;
-    }
-#pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      if (s >= count) break;
-      const uint32_t v = __shfl_sync(0xffffffffu, packed[s / 32], s % 32);
-      if (v != held) {
+    const int col = j + lane >= n ? j + lane - n : j + lane;
+    if (lane < w.count) w.f = pair_features(a, b0 + i0 + lane, b0 + col);
+  };
+  auto sum = [&](const Walk &w) {
+    if (w.count == 0) return;
+    const uint32_t packed = lane < w.count ? pick(a, w.f) : 0u;
+    const uint32_t first = __shfl_sync(0xffffffffu, packed, 0);
+    if (__all_sync(0xffffffffu, lane >= w.count || packed == first)) {  // one pick for the walk (rows past it are zero)
+      if (first != held) {
         if (held != 0xffffffffu) flush();
-        held = v;
+        held = first;
       }
-      if constexpr (sizeof(In) == 4)
-        run.x += x[s].x, run.y += x[s].y;
-      else
-        run.x += bf16_lo(x[s]), run.y += bf16_hi(x[s]);
+      float4 part = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kS; ++s) part = add4(part, as_float4(w.x[s]));
+      run = add4(run, part);
+    } else {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if (s < w.count) {
+          const uint32_t v = __shfl_sync(0xffffffffu, packed, s);
+          if (v != held) {
+            if (held != 0xffffffffu) flush();
+            held = v;
+          }
+          run = add4(run, as_float4(w.x[s]));
+        }
+      }
     }
+  };
+  const uint32_t hop = gridDim.x * groups;
+  Walk one, two;
+  uint32_t u = blockIdx.x * groups + group;
+  load(u, one);
+  for (; u < units; u += 2 * hop) {
+    load(u + hop, two);
+    sum(one);
+    load(u + 2 * hop, one);
+    sum(two);
   }
   if (held != 0xffffffffu) flush();
   __syncthreads();
@@ -238,7 +280,7 @@ __global__ void __launch_bounds__(256) encoding_grad_sum_kernel(const float *par
 
 int encoding_check(const char *name, const EncArgs &a, int64_t n, int64_t channels, int64_t r, int64_t s) {
   BL_REQUIRE(a.batch >= 0 && n >= 0 && n <= (1 << 15) && a.batch <= (1 << 20), "%s: bad shape", name);
-  BL_REQUIRE(a.batch * n * ((n + 31) / 32) < (int64_t(1) << 31), "%s: too many token pairs", name);
+  BL_REQUIRE(a.batch * n * ((n + 15) / 16) < (int64_t(1) << 30), "%s: too many token pairs", name);
   BL_REQUIRE(channels >= 4 && channels <= 4096 && channels % 4 == 0, "%s: channels must be a multiple of 4, at most 4096",
              name);
   BL_REQUIRE(r >= 0 && s >= 0 && r <= 96 && s <= 16, "%s: r_max must lie in [0, 96], s_max in [0, 16]", name);
@@ -251,7 +293,7 @@ int encoding_grad_groups(int rows) {  // private tables that fit in 227 KB
   return fit < kGroups ? fit : kGroups;
 }
 int64_t encoding_grad_ctas(int64_t batch, int64_t n, int rows, int chunks) {
-  const int64_t units = batch * ((n + 31) / 32) * n, groups = encoding_grad_groups(rows);
+  const int64_t units = batch * ((n + 15) / 16) * n, groups = encoding_grad_groups(rows);
   const int64_t want = (units + groups - 1) / groups, cap = (num_sms() + chunks - 1) / chunks;
   return want < 1 ? 1 : want < cap ? want : cap;
 }
@@ -274,57 +316,132 @@ __device__ __forceinline__ void load_lut(uint16_t *dst, const BiasArgs &a) {
     dst[i] = uint16_t(u < last ? u : last);
   }
 }
-__device__ __forceinline__ int bucket_of(const uint16_t *lut, const BiasArgs &a, int64_t q, int64_t k, bool same) {
-  const int64_t d = q - k;
-  const int at = d < -a.distance ? 0 : d > a.distance ? 2 * a.distance : int(d) + a.distance;
-  return same ? lut[at] : a.buckets - 1;
+// Four key columns of one sample.  Positions relative to the sample's first key and groups as 32
+// bits where they fit (`wide`: they do not, and are read again as 64 bits).
+constexpr int kFits = 1 << 29;
+struct Columns {
+  int k[4], g[4];
+  int64_t at;  // index of the first column
+  int count;   // columns that exist
+  bool wide;
+};
+__device__ __forceinline__ Columns load_columns(const BiasArgs &a, int64_t b, int j) {
+  Columns c;
+  c.at = b * a.nk + j;
+  c.count = a.nk - j < 4 ? a.nk - j : 4;
+  c.wide = false;
+  const int64_t base = a.k_pos[b * a.nk];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = c.at + (e < c.count ? e : 0), k = a.k_pos[at] - base, g = a.k_group ? a.k_group[at] : 0;
+    c.k[e] = int(k), c.g[e] = int(g);
+    c.wide |= k < -kFits || k > kFits || g != int64_t(int(g));
+  }
+  return c;
+}
+// Query rows [i0, i0 + rows) of sample b into shared memory: position relative to the sample's first
+// key as 32 bits (saturated: at least kFits from any key that fits), group, whether the group fits.
+__device__ __forceinline__ void load_rows_info(int4 *dst, const BiasArgs &a, int64_t b, int i0, int step, int rows) {
+  const int64_t base = a.k_pos[b * a.nk];
+  for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+    const int64_t at = b * a.nq + i0 + int64_t(r) * step, d = a.q_pos[at] - base, g = a.q_group ? a.q_group[at] : 0;
+    const int q = d < -2 * int64_t(kFits) ? -2 * kFits : d > 2 * int64_t(kFits) - 1 ? 2 * kFits - 1 : int(d);
+    dst[r] = make_int4(q, int(g), g == int64_t(int(g)), i0 + r * step);
+  }
+}
+// Buckets of one query row.
+__device__ __forceinline__ void buckets_of(int (&u)[4], const uint16_t *lut, const BiasArgs &a, const Columns &c, int64_t b,
+                                           const int4 &r) {
+  if (!c.wide) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = min(max(r.x - c.k[e], -a.distance), a.distance);
+      u[e] = lut[a.distance + at];
+      if (r.y != c.g[e] || !r.z) u[e] = a.buckets - 1;
+    }
+  } else {
+    const int64_t q = a.q_pos[b * a.nq + r.w], g = a.q_group ? a.q_group[b * a.nq + r.w] : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = c.at + (e < c.count ? e : 0), d = q - a.k_pos[at];
+      const int x = d < -a.distance ? 0 : d > a.distance ? 2 * a.distance : int(d) + a.distance;
+      u[e] = !a.k_group || g == a.k_group[at] ? int(lut[x]) : a.buckets - 1;
+    }
+  }
 }
 
 // A thread keeps four key columns and their positions, computes their buckets
 // once per query row and writes them for every head (16 or 8 bytes per store).
+// The table sits in shared memory as [bucket][heads + 4]: one 16-byte load gives a
+// column's value for four heads, and rows of different buckets start in different
+// banks (heads a multiple of 8, padded: 4 (heads / 4 + 1) words apart, odd multiples
+// of 4).  With [head][bucket] and a load per value the kernel took 28 instructions
+// per store and 115 us for 537 MB.
 constexpr int kBiasThreads = 128, kBiasCols = 4 * kBiasThreads;
+constexpr int kRowsPerCta = 4;
+constexpr int kBiasRows = 512;  // query rows whose positions sit in shared memory at a time
+
+__host__ __device__ inline int table_ld(int heads) { return (heads + 7) / 8 * 8 + 4; }
 
 template <typename Out>
-__global__ void __launch_bounds__(kBiasThreads) bias_kernel(const float *table, const BiasArgs a, Out *out, int q_rows,
-                                                            int vector) {
+__global__ void __launch_bounds__(kBiasThreads) bias_kernel(const float *table, const BiasArgs a, Out *out, int vector) {
   extern __shared__ float4 smem4[];
-  float *tab = reinterpret_cast<float *>(smem4);                      // [heads][buckets]
-  uint16_t *lut = reinterpret_cast<uint16_t *>(tab + a.heads * a.buckets);
-  for (int i = threadIdx.x; i < a.heads * a.buckets; i += kBiasThreads)
-    tab[i % a.heads * a.buckets + i / a.heads] = table[i];
+  const int ld = table_ld(a.heads);
+  int4 *info = reinterpret_cast<int4 *>(smem4);
+  float *tab = reinterpret_cast<float *>(info + kBiasRows);  // [buckets][ld]
+  uint16_t *lut = reinterpret_cast<uint16_t *>(tab + a.buckets * ld);
+  for (int i = threadIdx.x; i < a.heads * a.buckets; i += kBiasThreads) tab[i / a.heads * ld + i % a.heads] = table[i];
   load_lut(lut, a);
-  __syncthreads();
+  // blockIdx.x keeps its column block and walks the rows r, r + runs, ...: the rows that all CTAs
+  // write at a time are neighbours.
   const int64_t b = blockIdx.z;
   const int j = blockIdx.x * kBiasCols + 4 * threadIdx.x;
-  if (j >= a.nk) return;
-  const int count = a.nk - j < 4 ? a.nk - j : 4;
-  int64_t kp[4], kg[4];
+  const bool active = j < a.nk;
+  Columns c{};
+  if (active) c = load_columns(a, b, j);
+  const bool whole = vector && c.count == 4;
+  const int rows = (a.nq - int(blockIdx.y) + int(gridDim.y) - 1) / int(gridDim.y), full = a.heads & ~3;
+  for (int r0 = 0; r0 < rows; r0 += kBiasRows) {
+    const int now = rows - r0 < kBiasRows ? rows - r0 : kBiasRows;
+    __syncthreads();
+    load_rows_info(info, a, b, blockIdx.y + r0 * gridDim.y, gridDim.y, now);
+    __syncthreads();
+    if (!active) continue;
+    for (int t = 0; t < now; ++t) {
+      const int4 r = info[t];
+      int u[4];
+      buckets_of(u, lut, a, c, b, r);
+      const float *row[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t at = b * a.nk + j + (e < count ? e : 0);
-    kp[e] = a.k_pos[at];
-    kg[e] = a.k_group ? a.k_group[at] : 0;
-  }
-  const int i0 = blockIdx.y * q_rows, i1 = i0 + q_rows < a.nq ? i0 + q_rows : a.nq;
-  for (int i = i0; i < i1; ++i) {
-    const int64_t qp = a.q_pos[b * a.nq + i], qg = a.q_group ? a.q_group[b * a.nq + i] : 0;
-    int u[4];
+      for (int e = 0; e < 4; ++e) row[e] = tab + u[e] * ld;
+      Out *p = out + b * a.sb + int64_t(r.w) * a.sq + j;
+      auto four = [&](int h, float (&v)[4][4]) {  // [head][column]
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = bucket_of(lut, a, qp, kp[e], qg == kg[e]);
-    Out *p = out + b * a.sb + int64_t(i) * a.sq + j;
-    const float *row = tab;
+        for (int e = 0; e < 4; ++e) {
+          const float4 f = *reinterpret_cast<const float4 *>(row[e] + h);
+          v[0][e] = f.x, v[1][e] = f.y, v[2][e] = f.z, v[3][e] = f.w;
+        }
+      };
+      if (whole) {
 #pragma unroll 4
-    for (int h = 0; h < a.heads; ++h, row += a.buckets, p += a.sh) {
-      const float y[4] = {row[u[0]], row[u[1]], row[u[2]], row[u[3]]};
-      if (vector && count == 4) {
-        if constexpr (sizeof(Out) == 4)
-          __stcs(reinterpret_cast<float4 *>(p), make_float4(y[0], y[1], y[2], y[3]));
-        else
-          __stcs(reinterpret_cast<uint2 *>(p), make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])));
-      } else {
+        for (int h = 0; h < full; h += 4) {
+          float v[4][4];
+          four(h, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < count) store_from_float(p + e, y[e]);
+          for (int g = 0; g < 4; ++g, p += a.sh) put4(p, make_float4(v[g][0], v[g][1], v[g][2], v[g][3]));
+        }
+        if (full < a.heads) {
+          float v[4][4];
+          four(full, v);
+#pragma unroll
+          for (int g = 0; g < 3; ++g, p += a.sh)
+            if (full + g < a.heads) put4(p, make_float4(v[g][0], v[g][1], v[g][2], v[g][3]));
+        }
+      } else {
+        for (int h = 0; h < a.heads; ++h, p += a.sh)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < c.count) store_from_float(p + e, row[e][h]);
       }
     }
   }
@@ -334,8 +451,8 @@ __global__ void __launch_bounds__(kBiasThreads) bias_kernel(const float *table, 
 template <typename T> struct Quad;
 template <> struct Quad<float> {
   using type = float4;
-  static __device__ __forceinline__ float4 load(const float *p, int count, bool vector) {
-    if (vector) return __ldcs(reinterpret_cast<const float4 *>(p));
+  static __device__ __forceinline__ float4 load(const float *p) { return __ldcs(reinterpret_cast<const float4 *>(p)); }
+  static __device__ __forceinline__ float4 load_part(const float *p, int count) {
     return make_float4(p[0], count > 1 ? p[1] : 0.f, count > 2 ? p[2] : 0.f, count > 3 ? p[3] : 0.f);
   }
   static __device__ __forceinline__ float get(const float4 &v, int e) {
@@ -344,8 +461,10 @@ template <> struct Quad<float> {
 };
 template <> struct Quad<__nv_bfloat16> {
   using type = uint2;
-  static __device__ __forceinline__ uint2 load(const __nv_bfloat16 *p, int count, bool vector) {
-    if (vector) return __ldcs(reinterpret_cast<const uint2 *>(p));
+  static __device__ __forceinline__ uint2 load(const __nv_bfloat16 *p) {
+    return __ldcs(reinterpret_cast<const uint2 *>(p));
+  }
+  static __device__ __forceinline__ uint2 load_part(const __nv_bfloat16 *p, int count) {
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = e < count ? __bfloat162float(p[e]) : 0.f;
@@ -355,86 +474,83 @@ template <> struct Quad<__nv_bfloat16> {
     return e == 0 ? bf16_lo(v.x) : e == 1 ? bf16_hi(v.x) : e == 2 ? bf16_lo(v.y) : bf16_hi(v.y);
   }
 };
-
 // Gradient of the table.  A thread owns four key columns of kHeads heads and
 // walks down the query rows with one running sum per column and head; when a
 // column's bucket changes, its sums go to the thread's own column of the
 // shared histogram [bucket][head][thread] (bank = thread: no conflicts, no
 // atomics).  The bucket of a (row, column) is computed once for kHeads heads.
-template <typename In, int kHeads>
+// kVector: the four columns in one load (rows on 16-byte boundaries; 8 in bf16); else one by one.
+// One row at a time with enough warps per SM: two rows ahead in registers took 36 against 32 us at
+// 2 x 16 x 768 x 1024, and 67 against 45 us with unaligned rows (1134 keys).
+template <typename In, int kHeads, bool kVector>
 __global__ void __launch_bounds__(kBiasThreads) bias_grad_kernel(const In *grad, const BiasArgs a, int q_rows,
-                                                                 int vector, float *partial) {
+                                                                 float *partial) {
+  using Four = typename Quad<In>::type;
   extern __shared__ float4 smem4[];
-  float *hist = reinterpret_cast<float *>(smem4);
+  int4 *info = reinterpret_cast<int4 *>(smem4);
+  float *hist = reinterpret_cast<float *>(info + kBiasRows);
   uint16_t *lut = reinterpret_cast<uint16_t *>(hist + a.buckets * kHeads * kBiasThreads);
-  for (int i = threadIdx.x; i < a.buckets * kHeads * kBiasThreads; i += kBiasThreads) hist[i] = 0.f;
+  for (int i = threadIdx.x; i < a.buckets * kHeads * kBiasThreads / 4; i += kBiasThreads)
+    reinterpret_cast<float4 *>(hist)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   load_lut(lut, a);
-  __syncthreads();
   float *mine = hist + threadIdx.x;
   const int h0 = blockIdx.y * kHeads, heads = a.heads - h0 < kHeads ? a.heads - h0 : kHeads;
-  // Four columns per thread, consecutive over all samples: no thread idles at a row's end.
-  const int quads = (a.nk + 3) / 4, row_blocks = (a.nq + q_rows - 1) / q_rows;
-  const uint32_t all_quads = uint32_t(a.batch * quads), col_blocks = (all_quads + kBiasThreads - 1) / kBiasThreads;
-  const uint32_t units = col_blocks * row_blocks;
-  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const uint32_t rb = u / col_blocks, quad = (u - rb * col_blocks) * kBiasThreads + threadIdx.x;
-    if (quad >= all_quads) continue;
-    const int64_t b = quad / uint32_t(quads);
-    const int j = 4 * int(quad - uint32_t(b) * quads);
-    const int i0 = int(rb) * q_rows, i1 = i0 + q_rows < a.nq ? i0 + q_rows : a.nq;
-    const int count = a.nk - j < 4 ? a.nk - j : 4;
-    int64_t kp[4], kg[4];
+  // A sample's columns in equal blocks of at most 128 x 4.
+  const int quads = (a.nk + 3) / 4, col_blocks = (quads + kBiasThreads - 1) / kBiasThreads;
+  const int width = (quads + col_blocks - 1) / col_blocks, row_blocks = (a.nq + q_rows - 1) / q_rows;
+  const int64_t units = a.batch * col_blocks * row_blocks;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int rb = int(u % row_blocks), cb = int(u / row_blocks % col_blocks);
+    const int64_t b = u / row_blocks / col_blocks;
+    const int i0 = rb * q_rows, rows = a.nq - i0 < q_rows ? a.nq - i0 : q_rows;
+    const int j = 4 * (cb * width + int(threadIdx.x));
+    const bool active = int(threadIdx.x) < width && j < a.nk;
+    __syncthreads();
+    load_rows_info(info, a, b, i0, 1, rows);
+    __syncthreads();
+    if (!active) continue;
+    const Columns c = load_columns(a, b, j);
     int held[4];
     float run[4][kHeads];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t at = b * a.nk + j + (e < count ? e : 0);
-      kp[e] = a.k_pos[at];
-      kg[e] = a.k_group ? a.k_group[at] : 0;
       held[e] = -1;
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) run[e][h] = 0.f;
     }
-    const In *base = grad + b * a.sb + h0 * a.sh + j;
-    auto load = [&](int i, typename Quad<In>::type (&x)[kHeads]) {
+    auto take = [&](int r, const Four (&x)[kHeads]) {
+      int v[4];
+      buckets_of(v, lut, a, c, b, info[r]);
+      if (((v[0] ^ held[0]) | (v[1] ^ held[1]) | (v[2] ^ held[2]) | (v[3] ^ held[3])) != 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v[e] != held[e]) {
+            if (held[e] >= 0) {
+              float *to = mine + held[e] * kHeads * kBiasThreads;
+#pragma unroll
+              for (int h = 0; h < kHeads; ++h) {
+                to[h * kBiasThreads] += run[e][h];
+                run[e][h] = 0.f;
+              }
+            }
+            held[e] = v[e];
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) run[e][h] += Quad<In>::get(x[h], e);
+    };
+    const In *p = grad + b * a.sb + h0 * a.sh + int64_t(i0) * a.sq + j;
+    for (int t = 0; t < rows; ++t, p += a.sq) {
+      Four x[kHeads];
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
         x[h] = {};
-        if (h < heads) x[h] = Quad<In>::load(base + h * a.sh + int64_t(i) * a.sq, count, vector && count == 4);
+        if (h < heads)
+          x[h] = kVector && c.count == 4 ? Quad<In>::load(p + h * a.sh) : Quad<In>::load_part(p + h * a.sh, c.count);
       }
-    };
-    auto take = [&](int i, const typename Quad<In>::type (&x)[kHeads]) {
-      const int64_t qp = a.q_pos[b * a.nq + i], qg = a.q_group ? a.q_group[b * a.nq + i] : 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = bucket_of(lut, a, qp, kp[e], qg == kg[e]);
-        if (v != held[e]) {
-          if (held[e] >= 0) {
-#pragma unroll
-            for (int h = 0; h < kHeads; ++h) {
-              mine[(held[e] * kHeads + h) * kBiasThreads] += run[e][h];
-              run[e][h] = 0.f;
-            }
-          }
-          held[e] = v;
-        }
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) run[e][h] += Quad<In>::get(x[h], e);
-      }
-    };
-    constexpr int kAhead = 4;  // rows in flight
-    int i = i0;
-    for (; i + kAhead <= i1; i += kAhead) {
-      typename Quad<In>::type x[kAhead][kHeads];
-#pragma unroll
-      for (int r = 0; r < kAhead; ++r) load(i + r, x[r]);
-#pragma unroll
-      for (int r = 0; r < kAhead; ++r) take(i + r, x[r]);
-    }
-    for (; i < i1; ++i) {
-      typename Quad<In>::type x[kHeads];
-      load(i, x);
-      take(i, x);
+      take(t, x);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -445,12 +561,15 @@ __global__ void __launch_bounds__(kBiasThreads) bias_grad_kernel(const In *grad,
   }
   __syncthreads();
   // partial[head group][cta][bucket][kHeads]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // A thread sums a row of 128 in 16-byte steps, starting at a place of its own: no two lanes of a
+  // phase meet in a bank.
   float *dst = partial + (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets * kHeads;
-  for (int k = warp; k < a.buckets * kHeads; k += kBiasThreads / 32) {
-    const float *row = hist + k * kBiasThreads + lane;
-    const float v = warp_sum((row[0] + row[32]) + (row[64] + row[96]));
-    if (lane == 0) dst[k] = v;
+  for (int k = threadIdx.x; k < a.buckets * kHeads; k += kBiasThreads) {
+    const float4 *row = reinterpret_cast<const float4 *>(hist + k * kBiasThreads);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int e = 0; e < kBiasThreads / 4; ++e) v = add4(v, row[(e + k) % (kBiasThreads / 4)]);
+    dst[k] = (v.x + v.y) + (v.z + v.w);
   }
 }
 
@@ -482,8 +601,8 @@ int bias_check(const char *name, const BiasArgs &a) {
 
 int bias_lut_bytes(int distance) { return (2 * distance + 1) * 2; }
 int bias_grad_heads(int buckets) { return buckets <= 48 ? 4 : 1; }  // 2 KB (4 heads) or 0.5 KB (1) per bucket
-// Launch shape of the table gradient: three CTAs per SM (67 KB of histogram at 33 buckets x 4 heads), and rows per
-// unit such that a CTA has about eight units to even out, in whole groups of four rows.
+// Launch shape of the table gradient: up to three CTAs per SM (67 KB of histogram at 33 buckets x 4 heads), each with
+// one column block and one run of rows, in whole groups of four rows.
 struct BiasGrad {
   int per, groups, rows;
   int64_t ctas;
@@ -492,10 +611,12 @@ BiasGrad bias_grad_shape(int64_t batch, int64_t heads, int64_t nq, int64_t nk, i
   BiasGrad g;
   g.per = bias_grad_heads(buckets);
   g.groups = int((heads + g.per - 1) / g.per);
-  const int64_t cols = (batch * ((nk + 3) / 4) + kBiasThreads - 1) / kBiasThreads;
+  const int64_t cols = batch * (((nk + 3) / 4 + kBiasThreads - 1) / kBiasThreads);
   const int64_t cap = (3 * num_sms() + g.groups - 1) / g.groups;
-  int64_t rows = nq * cols / (8 * cap) / 4 * 4;
-  g.rows = int(rows < 4 ? 4 : rows > 64 ? 64 : rows);
+  int64_t runs = cap / cols;
+  runs = runs < 1 ? 1 : runs > (nq + 7) / 8 ? (nq + 7) / 8 : runs;
+  const int64_t rows = ((nq + runs - 1) / runs + 3) / 4 * 4;
+  g.rows = int(rows > kBiasRows ? kBiasRows : rows);
   const int64_t units = cols * ((nq + g.rows - 1) / g.rows);
   g.ctas = units < 1 ? 1 : units < cap ? units : cap;
   return g;
@@ -535,13 +656,15 @@ extern "C" int bl_relative_position_encoding(const float *weight, const int64_t 
   auto kernel16 = wide ? encoding_kernel<__nv_bfloat16, 32, false> : encoding_kernel<__nv_bfloat16, 8, false>;
   const void *fn = kernel ? reinterpret_cast<const void *>(kernel) : reinterpret_cast<const void *>(kernel16);
   BL_CUDA(ensure_smem_limit(fn, kMaxSmem));
-  const int64_t fit = kMaxSmem / (smem + 1024), per_sm = fit < 1 ? 1 : fit < 8 ? fit : 8;
-  const int64_t want = (units + 7) / 8, cap = (per_sm * num_sms() + chunks - 1) / chunks;
+  // One CTA per SM when wide: every CTA loads the table (71 KB), and three per SM spent 10 us at 512 tokens on it.
+  const int threads = wide ? 1024 : 256, warps = threads / 32;
+  const int64_t fit = kMaxSmem / (smem + 1024), per_sm = wide || fit < 1 ? 1 : fit < 8 ? fit : 8;
+  const int64_t want = (units + warps - 1) / warps, cap = (per_sm * num_sms() + chunks - 1) / chunks;
   dim3 grid(unsigned(want < cap ? want : cap), unsigned(chunks));
   if (kernel)
-    kernel<<<grid, 256, smem, as_stream(stream)>>>(weight, a, static_cast<float *>(out));
+    kernel<<<grid, threads, smem, as_stream(stream)>>>(weight, a, static_cast<float *>(out));
   else
-    kernel16<<<grid, 256, smem, as_stream(stream)>>>(weight, a, static_cast<__nv_bfloat16 *>(out));
+    kernel16<<<grid, threads, smem, as_stream(stream)>>>(weight, a, static_cast<__nv_bfloat16 *>(out));
   BL_LAUNCH_CHECK();
   return BL_OK;
 }
@@ -568,7 +691,7 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
     BL_CUDA(cudaMemsetAsync(dweight, 0, size_t(channels) * a.rows * 4, st));
     return BL_OK;
   }
-  BL_REQUIRE(grad && aligned_to(grad, dtype == BL_F32 ? 8 : 4),
+  BL_REQUIRE(grad && aligned_to(grad, dtype == BL_F32 ? 16 : 8),
              "bl_relative_position_encoding_backward: null or unaligned pointer");
   const int64_t need = bl_relative_position_encoding_workspace(batch, n, channels, r_max, s_max);
   BL_REQUIRE(workspace && workspace_bytes >= need && aligned_to(workspace, 16),
@@ -580,11 +703,11 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
   dim3 grid{unsigned(ctas), unsigned(chunks)};
   if (dtype == BL_F32) {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(encoding_grad_kernel<float>), kMaxSmem));
-    encoding_grad_kernel<float><<<grid, groups * 64, smem, st>>>(static_cast<const float *>(grad), a, part);
+    encoding_grad_kernel<float><<<grid, groups * 32, smem, st>>>(static_cast<const float *>(grad), a, part);
   } else {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(encoding_grad_kernel<__nv_bfloat16>), kMaxSmem));
     encoding_grad_kernel<__nv_bfloat16>
-        <<<grid, groups * 64, smem, st>>>(static_cast<const __nv_bfloat16 *>(grad), a, part);
+        <<<grid, groups * 32, smem, st>>>(static_cast<const __nv_bfloat16 *>(grad), a, part);
   }
   BL_LAUNCH_CHECK();
   const int64_t size = int64_t(chunks) * a.rows * 128;
@@ -606,22 +729,23 @@ extern "C" int bl_relative_position_bias(const float *table, const int64_t *q_po
   BL_REQUIRE(out_dtype == BL_F32 || out_dtype == BL_BF16, "bl_relative_position_bias: dtype must be fp32 or bf16");
   if (batch == 0 || nq == 0 || nk == 0) return BL_OK;
   BL_REQUIRE(table && out, "bl_relative_position_bias: null pointer");
-  const int smem = a.heads * a.buckets * 4 + bias_lut_bytes(a.distance);
+  const int smem = kBiasRows * 16 + table_ld(a.heads) * a.buckets * 4 + bias_lut_bytes(a.distance);
   const int64_t col_blocks = (nk + kBiasCols - 1) / kBiasCols;
-  // Query rows per CTA: about eight CTAs per SM in all, at most 32 rows each.
-  const int64_t want = 8 * int64_t(num_sms());
-  int64_t rows = (nq * col_blocks * batch + want - 1) / want;
-  rows = rows < 1 ? 1 : rows > 32 ? 32 : rows;
-  while ((nq + rows - 1) / rows > 65535) rows *= 2;
-  dim3 grid{unsigned(col_blocks), unsigned((nq + rows - 1) / rows), unsigned(batch)};
+  // Four rows per CTA, fewer while that leaves SMs without eight CTAs.  (Long runs of rows write in
+  // many places at once: filling the planes alone takes 90 us in runs of 28 rows, 77 us row by row.)
+  const int64_t least = 8 * int64_t(num_sms()) / (col_blocks * batch);
+  int64_t runs = (nq + kRowsPerCta - 1) / kRowsPerCta;
+  runs = runs < least ? (least < nq ? least : nq) : runs;
+  runs = runs > 65535 ? 65535 : runs;
+  dim3 grid{unsigned(col_blocks), unsigned(runs), unsigned(batch)};
   const int vec = vector_planes(out, a, out_dtype);
   if (out_dtype == BL_F32) {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(bias_kernel<float>), kMaxSmem));
-    bias_kernel<float><<<grid, kBiasThreads, smem, as_stream(stream)>>>(table, a, static_cast<float *>(out), int(rows), vec);
+    bias_kernel<float><<<grid, kBiasThreads, smem, as_stream(stream)>>>(table, a, static_cast<float *>(out), vec);
   } else {
     BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(bias_kernel<__nv_bfloat16>), kMaxSmem));
     bias_kernel<__nv_bfloat16>
-        <<<grid, kBiasThreads, smem, as_stream(stream)>>>(table, a, static_cast<__nv_bfloat16 *>(out), int(rows), vec);
+        <<<grid, kBiasThreads, smem, as_stream(stream)>>>(table, a, static_cast<__nv_bfloat16 *>(out), vec);
   }
   BL_LAUNCH_CHECK();
   return BL_OK;
@@ -658,20 +782,22 @@ extern "C" int bl_relative_position_bias_backward(const void *grad, int dtype, i
   const BiasGrad shape = bias_grad_shape(batch, heads, nq, nk, a.buckets);
   const int per = shape.per, groups = shape.groups, rows = shape.rows;
   const int64_t ctas = shape.ctas;
-  const int smem = a.buckets * per * kBiasThreads * 4 + bias_lut_bytes(a.distance);
+  const int smem = kBiasRows * 16 + a.buckets * per * kBiasThreads * 4 + bias_lut_bytes(a.distance);
   float *part = static_cast<float *>(workspace);
   const int vec = vector_planes(grad, a, dtype);
   dim3 grid{unsigned(ctas), unsigned(groups)};
-#define BL_BIAS_GRAD(T, K)                                                                                        \
-  do {                                                                                                            \
-    BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(bias_grad_kernel<T, K>), kMaxSmem));                     \
-    bias_grad_kernel<T, K><<<grid, kBiasThreads, smem, st>>>(static_cast<const T *>(grad), a, rows, vec, part);   \
+#define BL_BIAS_GRAD(T, K, V)                                                                                   \
+  do {                                                                                                          \
+    BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(bias_grad_kernel<T, K, V>), kMaxSmem));            \
+    bias_grad_kernel<T, K, V><<<grid, kBiasThreads, smem, st>>>(static_cast<const T *>(grad), a, rows, part);   \
   } while (0)
-  if (dtype == BL_F32) {
-    if (per == 4) BL_BIAS_GRAD(float, 4); else BL_BIAS_GRAD(float, 1);
-  } else {
-    if (per == 4) BL_BIAS_GRAD(__nv_bfloat16, 4); else BL_BIAS_GRAD(__nv_bfloat16, 1);
-  }
+#define BL_BIAS_GRAD_BY(T)                                                                                      \
+  do {                                                                                                          \
+    if (per == 4) { if (vec) BL_BIAS_GRAD(T, 4, true); else BL_BIAS_GRAD(T, 4, false); }                        \
+    else { if (vec) BL_BIAS_GRAD(T, 1, true); else BL_BIAS_GRAD(T, 1, false); }                                 \
+  } while (0)
+  if (dtype == BL_F32) BL_BIAS_GRAD_BY(float); else BL_BIAS_GRAD_BY(__nv_bfloat16);
+#undef BL_BIAS_GRAD_BY
 #undef BL_BIAS_GRAD
   BL_LAUNCH_CHECK();
   bias_grad_sum_kernel<<<unsigned((a.buckets * a.heads + 7) / 8), 256, 0, st>>>(part, int(ctas), a.buckets, a.heads, per,

@@ -475,7 +475,7 @@ def relative_position_encoding_backward(grad, residue_index, asym_id, entity_id,
     features = _indices(device, (b, n), residue_index=residue_index, asym_id=asym_id, entity_id=entity_id,
                         token_index=token_index, sym_id=sym_id)
     grad = grad.contiguous()
-    if grad.data_ptr() % 8:
+    if grad.data_ptr() % 16:
         grad = grad.clone()
     dweight = torch.empty(c, relative_position_columns(r_max, s_max), device=device, dtype=torch.float32)
     nbytes = size_of("bl_relative_position_encoding_workspace", b, n, c, r_max, s_max)
