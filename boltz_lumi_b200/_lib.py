@@ -7,6 +7,7 @@ and turns a non-zero status into ``RuntimeError`` carrying ``bl_last_error()``.
 """
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 
@@ -30,6 +31,12 @@ class CrossAttentionArgs(ctypes.Structure):
                 + [(n, c_int64) for n in ("mask_stride", "bias_share", "batch", "heads", "kv_heads", "nq", "nk", "head_dim")]
                 + [("out", c_void_p), ("low", c_void_p), ("lse", c_void_p), ("scale", c_float), ("inf", c_float), ("dtype", c_int),
                    ("mask_kind", c_int)])
+
+    # The same fields for one pack_into: an assignment per field costs more than the launch.
+    PACKING = struct.Struct("@6P15q8q3P2f2i")
+
+
+assert CrossAttentionArgs.PACKING.size == ctypes.sizeof(CrossAttentionArgs)
 
 
 _xargs = ctypes.POINTER(CrossAttentionArgs)
@@ -165,6 +172,10 @@ def call(name, *args):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+# torch.cuda.current_device() without its initialisation check (the caller holds a CUDA tensor).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_of(tensor: torch.Tensor) -> int:
     """Raw handle of torch's current stream on the tensor's device."""
     if _raw_stream is not None:
@@ -183,7 +194,7 @@ def current_stream_handle() -> int:
 def launch(device, name, *args):
     """:func:`call` ``name(*args, stream)`` on torch's current stream of ``device``, whichever device is current."""
     index = device.index
-    current = torch.cuda.current_device()
+    current = _current_device()
     if index is None or index == current:
         return call(name, *args, _raw_stream(current) if _raw_stream is not None else current_stream_handle())
     with torch.cuda.device(device):
@@ -192,7 +203,10 @@ def launch(device, name, *args):
 
 def size_of(name, *args):
     """The value of a size query of the library (no status, no launch)."""
-    return getattr(load(), name)(*args)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    return fn(*args)
 
 
 def ptr(tensor):

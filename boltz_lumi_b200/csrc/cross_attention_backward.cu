@@ -9,7 +9,7 @@
 //   rows_kernel    one pass over dy and out: delta, do, dgate.  Where one key dominates a
 //                  row, do . v and delta cancel, so in bf16 both need more than 8 bits: delta
 //                  takes out with the part that its rounding took (`low`), and a gated do
-//                  goes into do . v as two bf16 terms;
+//                  goes into do . v (and dv, whose p is rounded already) as two bf16 terms;
 //   keys_kernel    one CTA = 64 keys of one (sample, key/value head): dk and dv,
 //                  summed over the query tiles of every head that shares them;
 //   queries_kernel one CTA = up to 64 query rows of one (sample, head): dq, and
@@ -182,6 +182,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
         grad_score(s[n][2], dp[n][2], a.scale, bv[2], mk[1], m0, n0, dl.x);
         grad_score(s[n][3], dp[n][3], a.scale, bv[3], mk[1], m1, n1, dl.y);
       }
+      if (x.dlow) mma_acc<NT, DP>(dv, s, dls + buf * BQ * ld, lane);
       mma_acc<NT, DP>(dv, s, dt, lane);
       mma_acc<NT, DP>(dk, dp, qt, lane);
     }

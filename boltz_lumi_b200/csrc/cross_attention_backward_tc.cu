@@ -6,12 +6,12 @@
 //                      dQ += dS K; dS itself is the bias gradient where no sample shares the bias.
 //   keys_tc_kernel     one CTA = 128 keys of one (sample, key/value head) over query tiles of 64 of
 //                      every head that reads them: S^T = K Q^T and dP^T = V dO^T, P^T and dS^T as
-//                      bf16 in TMEM, dV += P^T dO, dK += dS^T Q.
+//                      bf16 in TMEM, dV += P^T dO, dK += dS^T Q (a gated dO in two bf16 terms).
 //
 // Both: warp 0 feeds the tiles by TMA, warp 1 issues the MMAs, warps 4..11 own half a TMEM lane's
 // columns per thread (lane = the resident row).  A tile's scores go to registers at once, so the
 // next tile's products run under this tile's arithmetic.  There is no row maximum to agree on:
-// the forward's statistics give p directly.  A gated do enters dP as two bf16 terms.
+// the forward's statistics give p directly.  A gated do enters dP and dV as two bf16 terms.
 // Against the same loops on mma.sync (measured in cross_attention_backward.cu's comment) they
 // gain because the 16-row warp products there re-read every operand tile from shared memory
 // once per 16 rows.
@@ -442,6 +442,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         for (int e = 0; e < kTileTc / 16; ++e)
           tc::umma_f16_ts(tmem + kDvCol, tmem + kPtCol + (u & 1) * 32 + e * 8, tc::desc_sw128(d + e * 2048, kTileTc * 128),
                           idesc_d, (u | e) != 0);
+        if (kLow)
+#pragma unroll
+          for (int e = 0; e < kTileTc / 16; ++e)
+            tc::umma_f16_ts(tmem + kDvCol, tmem + kPtCol + (u & 1) * 32 + e * 8,
+                            tc::desc_sw128(d + S::kStr + e * 2048, kTileTc * 128), idesc_d, true);
 #pragma unroll
         for (int e = 0; e < kTileTc / 16; ++e)
           tc::umma_f16_ts(tmem + kDkCol, tmem + kDstCol + (u & 1) * 32 + e * 8, tc::desc_sw128(q + e * 2048, kTileTc * 128),

@@ -18,8 +18,10 @@ from ._lib import call, launch, ptr, size_of, stream_of
 
 
 def _require_inference(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("boltz_lumi_b200 kernels are inference-only (grad mode with requires_grad inputs)")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("boltz_lumi_b200 kernels are inference-only (grad mode with requires_grad inputs)")
 
 
 def _require_cuda(*tensors):
@@ -400,12 +402,13 @@ def _indices(device, shape, **tensors):
         if t is not None:
             if t.device != device:
                 raise RuntimeError(f"{name} must be on {device}, got {t.device}")
-            if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
-                raise RuntimeError(f"{name} must hold integers, got {t.dtype}")
-            if tuple(t.shape) != tuple(shape):
+            if t.shape != shape:
                 raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-            if t.dtype != torch.int64 or not t.is_contiguous():
-                t = t.to(torch.int64).contiguous()
+            if t.dtype != torch.int64:
+                if t.dtype not in (torch.int32, torch.int16, torch.uint8):
+                    raise RuntimeError(f"{name} must hold integers, got {t.dtype}")
+                t = t.to(torch.int64)
+            t = t.contiguous()
         out.append(t)
     return out
 
@@ -456,7 +459,7 @@ def relative_position_encoding(weight, residue_index, asym_id, entity_id, token_
     else:
         out = torch.empty(b, n, n, c, device=weight.device, dtype=_float_dtype(out_dtype or torch.float32, "out_dtype"))
     weight = weight.contiguous()
-    launch(weight.device, "bl_relative_position_encoding", weight.data_ptr(), *(t.data_ptr() for t in features), b, n, c,
+    launch(weight.device, "bl_relative_position_encoding", weight.data_ptr(), *[t.data_ptr() for t in features], b, n, c,
            r_max, s_max, int(fix_sym_check), out.data_ptr(), _lib.dtype_code(out.dtype), int(residual is not None))
     return out
 
@@ -481,7 +484,7 @@ def relative_position_encoding_backward(grad, residue_index, asym_id, entity_id,
     nbytes = size_of("bl_relative_position_encoding_workspace", b, n, c, r_max, s_max)
     work = _workspace(nbytes, device)
     launch(device, "bl_relative_position_encoding_backward", grad.data_ptr(), _lib.dtype_code(grad.dtype),
-           *(t.data_ptr() for t in features), b, n, c, r_max, s_max, int(fix_sym_check), dweight.data_ptr(),
+           *[t.data_ptr() for t in features], b, n, c, r_max, s_max, int(fix_sym_check), dweight.data_ptr(),
            work.data_ptr(), nbytes)
     return dweight
 
@@ -597,6 +600,9 @@ def _attention_rows(t, dtype, name, shape):
     return t
 
 
+_NO_STRIDES = (0, 0, 0)
+
+
 def _attention_args(q, k, v, bias, mask, inf, gate, scale):
     """(the filled argument structure, the tensors it points into)."""
     device = _require_cuda(q, k, v, bias, mask, gate)
@@ -612,14 +618,12 @@ def _attention_args(q, k, v, bias, mask, inf, gate, scale):
     q = _attention_rows(q, dtype, "q", (b, nq, h, d))
     k = _attention_rows(k, dtype, "k", (b, nk, hk, d))
     v = _attention_rows(v, dtype, "v", (b, nk, hk, d))
-    x = _lib.CrossAttentionArgs()
-    x.q, x.k, x.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    x.q_stride[:], x.k_stride[:], x.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    gate_ptr = bias_ptr = mask_ptr = 0
+    gate_stride = bias_stride = _NO_STRIDES
+    share, mask_stride, mask_kind = 1, 0, 0
     if gate is not None:
         gate = _attention_rows(gate, dtype, "gate", (b, nq, h, d))
-        x.gate = gate.data_ptr()
-        x.gate_stride[:] = gate.stride()[:3]
-    x.bias_share = 1
+        gate_ptr, gate_stride = gate.data_ptr(), gate.stride()
     if bias is not None:
         if bias.dtype != dtype or bias.dim() != 4 or tuple(bias.shape[1:]) != (h, nq, nk) or bias.shape[0] < 1 \
                 or b % bias.shape[0]:
@@ -628,25 +632,25 @@ def _attention_args(q, k, v, bias, mask, inf, gate, scale):
         if bias.stride(3) != 1 and nk > 1:
             planes = padded_planes(*bias.shape, device, dtype)
             bias = planes.copy_(bias)
-        x.bias = bias.data_ptr()
-        x.bias_stride[:] = bias.stride()[:3]
-        x.bias_share = b // bias.shape[0]
+        bias_ptr, bias_stride, share = bias.data_ptr(), bias.stride(), b // bias.shape[0]
     if mask is not None:
         if tuple(mask.shape) != (b, nk):
             raise RuntimeError(f"mask must be [{b}, {nk}], got {list(mask.shape)}")
         if inf is None:
             if mask.dtype != torch.bool:
                 raise RuntimeError("a mask without inf must be bool (True: the key is kept)")
-            x.mask_kind = 1
+            mask_kind = 1
         else:
             mask = mask.float()
-            x.mask_kind, x.inf = 2, float(inf)
+            mask_kind = 2
         if mask.stride(1) != 1 and nk > 1:
             mask = mask.contiguous()
-        x.mask, x.mask_stride = mask.data_ptr(), mask.stride(0)
-    x.batch, x.heads, x.kv_heads, x.nq, x.nk, x.head_dim = b, h, hk, nq, nk, d
-    x.scale = d ** -0.5 if scale is None else float(scale)
-    x.dtype = _lib.dtype_code(dtype)
+        mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0)
+    x = _lib.CrossAttentionArgs()
+    x.PACKING.pack_into(x, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), gate_ptr, bias_ptr, mask_ptr, *q.stride()[:3],
+                        *k.stride()[:3], *v.stride()[:3], *gate_stride[:3], *bias_stride[:3], mask_stride, share,
+                        b, h, hk, nq, nk, d, 0, 0, 0, d ** -0.5 if scale is None else scale,
+                        inf if mask_kind == 2 else 0.0, _lib.dtype_code(dtype), mask_kind)
     return x, (q, k, v, bias, mask, gate)
 
 
