@@ -35,17 +35,20 @@ template <int kBlocks, bool kBias, bool kLow> struct QShape {
   static constexpr int kRes = kRowsTc * 128 * kBlocks;  // bytes of a resident 128-row tile
   static constexpr int kStr = kTileTc * 128 * kBlocks;  // bytes of a streamed 64-row tile
   static constexpr int kB = kBias ? kRowsTc * kTileTc * 2 : 0;
-  static constexpr int kStages = kBlocks == 2 && kLow && kBias ? 2 : 3, kBiasStages = 2;
-  static constexpr int kResident = kLow ? 3 : 2;        // Q, dO, do - bf16(do)
-  static constexpr int kStrOff = kResident * kRes;      // [stage]{K, V}
-  static constexpr int kBiasOff = kStrOff + kStages * 2 * kStr;
-  static constexpr int kMaskOff = kBiasOff + kBiasStages * kB;  // [warp][32] additive mask values
+  // A tile's load takes about as long as two tiles' arithmetic: K, which dQ still reads, needs the
+  // longest ring, V is free after dP.
+  static constexpr int kKStages = kBlocks == 1 ? 6 : kLow && kBias ? 3 : kLow || kBias ? 4 : 5;
+  static constexpr int kVStages = kKStages - 1, kBiasStages = kBlocks == 1 ? 4 : 2;
+  static constexpr int kResident = kLow ? 3 : 2;  // Q, dO, do - bf16(do)
+  static constexpr int kKOff = kResident * kRes, kVOff = kKOff + kKStages * kStr;
+  static constexpr int kBiasOff = kVOff + kVStages * kStr;
+  static constexpr int kMaskOff = kBiasOff + (kBias ? kBiasStages * kB : 0);  // [warp][32] additive mask values
   static constexpr int kBitsOff = kMaskOff + 8 * 32 * 4;
   static constexpr int kBarOff = kBitsOff + kMaskWords * 4;
-  static constexpr int kBytes = kBarOff + 256 + 1024;
+  static constexpr int kBytes = kBarOff + 512 + 1024;
 };
-// TMEM columns: S, dP (64 each), two dS buffers (32 each), dQ.
-constexpr uint32_t kSCol = 0, kDpCol = 64, kDsCol = 128, kDqCol = 256;
+// TMEM columns: two buffers of S and dP (64 each), two of dS (32 each), dQ.
+constexpr uint32_t kSCol = 0, kDpCol = 64, kPair = 128, kDsCol = 256, kDqCol = 320;
 
 template <int kBlocks, bool kBias, bool kLow>
 __global__ void __launch_bounds__(kThreadsTc, 1)
@@ -54,18 +57,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias,
                       const BackTc p) {
   using S = QShape<kBlocks, kBias, kLow>;
-  constexpr int ST = S::kStages, BS = S::kBiasStages;
+  constexpr int KS = S::kKStages, VS = S::kVStages, BS = S::kBiasStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
   uint64_t *res_full = bars;             // resident tiles landed
-  uint64_t *st_full = res_full + 1;      // [ST] K and V of a key tile landed
-  uint64_t *st_empty = st_full + ST;     // [ST] dQ has read that K
-  uint64_t *b_full = st_empty + ST;      // [BS] bias block landed
+  uint64_t *k_full = res_full + 1;       // [KS] K of a key tile landed
+  uint64_t *k_empty = k_full + KS;       // [KS] dQ has read it
+  uint64_t *v_full = k_empty + KS;       // [VS] V landed
+  uint64_t *v_empty = v_full + VS;       // [VS] dP has read it
+  uint64_t *b_full = v_empty + VS;       // [BS] bias block landed
   uint64_t *b_empty = b_full + BS;       // [BS] it has been read
-  uint64_t *s_full = b_empty + BS;       // S and dP in TMEM
-  uint64_t *s_free = s_full + 1;         // they are in registers
-  uint64_t *ds_full = s_free + 1;        // [2] dS in TMEM
+  uint64_t *s_full = b_empty + BS;       // [2] S and dP in TMEM
+  uint64_t *ds_full = s_full + 2;        // [2] they have been read, dS is in TMEM
   uint64_t *dq_full = ds_full + 2;       // every product is done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(dq_full + 1);
   int *last_key = reinterpret_cast<int *>(tmem_slot + 1);
@@ -76,10 +80,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   const int q0 = tile * kRowsTc, hk = h / a.group, bb = b / a.share;
   if (tid == 0) {
     tc::mbar_init(res_full, 1);
-    for (int i = 0; i < ST; ++i) tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1);
-    for (int i = 0; i < BS; ++i) tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 8);
-    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8), tc::mbar_init(dq_full, 1);
-    tc::mbar_init(ds_full, 8), tc::mbar_init(ds_full + 1, 8);
+    for (int i = 0; i < KS; ++i) tc::mbar_init(k_full + i, 1), tc::mbar_init(k_empty + i, 1);
+    for (int i = 0; i < VS; ++i) tc::mbar_init(v_full + i, 1), tc::mbar_init(v_empty + i, 1);
+    for (int i = 0; i < BS; ++i) tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 4);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(s_full + i, 2), tc::mbar_init(ds_full + i, 4);
+    tc::mbar_init(dq_full, 1);
     tc::fence_mbar_init();
     *last_key = -1;
   }
@@ -117,63 +122,69 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         tma_load_4d(smem + S::kRes + c * kRowsTc * 128, &map_do, res_full, 64 * c, q0, h, b);
         if (kLow) tma_load_4d(smem + 2 * S::kRes + c * kRowsTc * 128, &map_low, res_full, 64 * c, q0, h, b);
       }
-      bool ok = true;
       for (int j = 0; j < n; ++j) {
-        const int s = j % ST;
-        if (j >= ST && !(ok = wait_phase(st_empty + s, ((j / ST) & 1) ^ 1u, p.status, 0x401))) break;
-        uint8_t *st = smem + S::kStrOff + s * 2 * S::kStr;
-        tc::mbar_arrive_expect_tx(st_full + s, 2 * S::kStr);
-        for (int c = 0; c < kBlocks; ++c) {
-          tma_load_4d(st + c * kTileTc * 128, &map_k, st_full + s, 64 * c, j * kTileTc, hk, b);
-          tma_load_4d(st + S::kStr + c * kTileTc * 128, &map_v, st_full + s, 64 * c, j * kTileTc, hk, b);
-        }
+        const int ks = j % KS, vs = j % VS;
+        if (j >= KS && !wait_phase(k_empty + ks, ((j / KS) & 1) ^ 1u, p.status, 0x401)) break;
+        tc::mbar_arrive_expect_tx(k_full + ks, S::kStr);
+        for (int c = 0; c < kBlocks; ++c)
+          tma_load_4d(smem + S::kKOff + ks * S::kStr + c * kTileTc * 128, &map_k, k_full + ks, 64 * c, j * kTileTc, hk, b);
+        if (j >= VS && !wait_phase(v_empty + vs, ((j / VS) & 1) ^ 1u, p.status, 0x40B)) break;
+        tc::mbar_arrive_expect_tx(v_full + vs, S::kStr);
+        for (int c = 0; c < kBlocks; ++c)
+          tma_load_4d(smem + S::kVOff + vs * S::kStr + c * kTileTc * 128, &map_v, v_full + vs, 64 * c, j * kTileTc, hk, b);
         if constexpr (kBias) {
           const int bs = j % BS;
-          if (j >= BS && !(ok = wait_phase(b_empty + bs, ((j / BS) & 1) ^ 1u, p.status, 0x402))) break;
+          if (j >= BS && !wait_phase(b_empty + bs, ((j / BS) & 1) ^ 1u, p.status, 0x402)) break;
           tc::mbar_arrive_expect_tx(b_full + bs, S::kB);
           tma_load_4d(smem + S::kBiasOff + bs * S::kB, &map_bias, b_full + bs, j * kTileTc, q0, h, bb);
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp < 3) {
+    // ---------------- S (warp 1) and dP (warp 2), two tiles ahead of dQ ----------------
     if (lane == 0 && n > 0 && wait_phase(res_full, 0, p.status, 0x403)) {
       constexpr uint32_t idesc_s = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
-      const int steps = (a.d + 15) / 16;
-      const uint32_t idesc_dq = tc::idesc_bf16(kRowsTc, 16 * steps, false, true);
-      const uint32_t base = smem_addr(smem);
-      auto product = [&](uint32_t col, uint32_t res, uint32_t str, bool add) {  // resident rows . streamed rows
-        for (int e = 0; e < steps; ++e)
-          tc::umma_f16_ss(tmem + col, desc_k(res + (e >> 2) * kRowsTc * 128 + (e & 3) * 32),
-                          desc_k(str + (e >> 2) * kTileTc * 128 + (e & 3) * 32), idesc_s, add || e != 0);
-      };
-      auto issue = [&](int j) {
-        const int s = j % ST;
-        if (!wait_phase(st_full + s, (j / ST) & 1, p.status, 0x404)) return false;
-        if (j > 0 && !wait_phase(s_free, (j - 1) & 1, p.status, 0x405)) return false;
+      const uint32_t base = low_k(smem_addr(smem));
+      for (int j = 0; j < n; ++j) {
+        const int set = j & 1, st = warp == 1 ? j % KS : j % VS;
+        // This buffer's scores are in registers.
+        if (j >= 2 && !wait_phase(ds_full + set, ((j - 2) >> 1) & 1, p.status, 0x404)) break;
+        if (warp == 1) {
+          if (!wait_phase(k_full + st, (j / KS) & 1, p.status, 0x405)) break;
+          tc::tc_fence_after();
+          mma_rows_ss<kBlocks>(tmem + set * kPair + kSCol, base, kRowsTc * 128, base + ((S::kKOff + st * S::kStr) >> 4),
+                               kTileTc * 128, idesc_s, false);
+          tc::umma_commit(s_full + set);
+        } else {
+          if (!wait_phase(v_full + st, (j / VS) & 1, p.status, 0x406)) break;
+          tc::tc_fence_after();
+          const uint32_t v = base + ((S::kVOff + st * S::kStr) >> 4);
+          mma_rows_ss<kBlocks>(tmem + set * kPair + kDpCol, base + (S::kRes >> 4), kRowsTc * 128, v, kTileTc * 128, idesc_s, false);
+          if (kLow)
+            mma_rows_ss<kBlocks>(tmem + set * kPair + kDpCol, base + (2 * S::kRes >> 4), kRowsTc * 128, v, kTileTc * 128, idesc_s,
+                                 true);
+          tc::umma_commit(s_full + set);
+          tc::umma_commit(v_empty + st);
+        }
+      }
+    }
+  } else if (warp == 3) {
+    if (lane == 0) {
+      const uint32_t idesc_dq = tc::idesc_bf16(kRowsTc, (a.d + 15) / 16 * 16, false, true);
+      const uint32_t base = low_mn(smem_addr(smem), kTileTc * 128);
+      for (int j = 0; j < n; ++j) {
+        const int ks = j % KS;
+        if (!wait_phase(ds_full + (j & 1), (j >> 1) & 1, p.status, 0x40C) || !wait_phase(k_full + ks, (j / KS) & 1, p.status, 0x40D))
+          break;
         tc::tc_fence_after();
-        const uint32_t k = base + S::kStrOff + s * 2 * S::kStr, v = k + S::kStr;
-        product(kSCol, base, k, false);
-        product(kDpCol, base + S::kRes, v, false);
-        if (kLow) product(kDpCol, base + 2 * S::kRes, v, true);
-        tc::umma_commit(s_full);
-        return true;
-      };
-      bool ok = issue(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n && !(ok = issue(j + 1))) break;
-        if (!(ok = wait_phase(ds_full + (j & 1), (j >> 1) & 1, p.status, 0x406))) break;
-        tc::tc_fence_after();
-        const uint32_t k = base + S::kStrOff + (j % ST) * 2 * S::kStr;
-#pragma unroll
-        for (int e = 0; e < kTileTc / 16; ++e)
-          tc::umma_f16_ts(tmem + kDqCol, tmem + kDsCol + (j & 1) * 32 + e * 8, tc::desc_sw128(k + e * 2048, kTileTc * 128),
-                          idesc_dq, (j | e) != 0);
-        tc::umma_commit(st_empty + j % ST);
+        mma_cols_ts<kTileTc / 16>(tmem + kDqCol, tmem + kDsCol + (j & 1) * 32, base + ((S::kKOff + ks * S::kStr) >> 4), idesc_dq,
+                                  j != 0);
+        tc::umma_commit(k_empty + ks);
         if (j + 1 == n) tc::umma_commit(dq_full);
       }
     }
   } else if (warp >= 4) {
-    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = q0 + row;
+    const int set = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, i = q0 + row;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
     float *mk = reinterpret_cast<float *>(smem + S::kMaskOff) + (warp - 4) * 32;
     float m = INFINITY, nl = 0.f, delta = 0.f;
@@ -189,7 +200,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     ? static_cast<Bf *>(p.x.dbias) + ((int64_t(b) * a.heads + h) * a.nq + i) * p.x.dbias_ld
                     : nullptr;
     bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
+    for (int j = set; j < n && ok; j += 2) {
+      const int bs = j % BS;
+#pragma unroll 1
+      for (int half = 0; half < 2 && ok; ++half) {
       const int k0 = j * kTileTc + 32 * half;
       uint32_t cut = 0;
       if (a.mask_kind == kMaskNone) {
@@ -208,18 +222,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         cut = __ballot_sync(0xffffffffu, v == -INFINITY);  // from here on: keys that count nothing
         __syncwarp();
       }
-      if (!(ok = warp_wait(s_full, j & 1, p.status, 0x407))) break;
-      tc::tc_fence_after();
+      if (half == 0) {
+        if (!(ok = warp_wait(s_full + set, (j >> 1) & 1, p.status, 0x407))) break;
+        tc::tc_fence_after();
+        if constexpr (kBias) ok = warp_wait(b_full + bs, (j / BS) & 1, p.status, 0x408);
+        if (!ok) break;
+      }
       uint32_t sv[32], dv[32];
-      tc::tmem_ld_32x32b_x32(lanes + kSCol + 32 * half, sv);
-      tc::tmem_ld_32x32b_x32(lanes + kDpCol + 32 * half, dv);
-      const int bs = j % BS;
-      if constexpr (kBias) ok = warp_wait(b_full + bs, (j / BS) & 1, p.status, 0x408);
+      tc::tmem_ld_32x32b_x32(lanes + set * kPair + kSCol + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(lanes + set * kPair + kDpCol + 32 * half, dv);
       tc::tmem_ld_wait_regs(sv, dv);
-      if (!ok) break;
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(s_free);
       uint64_t y[16];
       if constexpr (kBias) {
         const uint32_t brow = smem_addr(smem + S::kBiasOff + bs * S::kB) + row * 128;
@@ -232,7 +244,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             y[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
         }
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(b_empty + bs);
+        if (half == 1 && lane == 0) tc::mbar_arrive(b_empty + bs);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
@@ -260,10 +272,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         }
         // K rows of left-out keys must be zero before dS meets them in dQ.
         if (a.mask_kind == kMaskKeep) {
-          const int s = j % ST, key = 8 * quarter + (lane >> 2);
+          const int ks = j % KS, key = 8 * quarter + (lane >> 2);
           if (cut >> key & 1) {
-            wait_phase(st_full + s, (j / ST) & 1, p.status, 0x409);  // complete: S came from this stage
-            uint8_t *k = smem + S::kStrOff + s * 2 * S::kStr + (32 * half + key) * 128 + (lane & 3) * 32;
+            wait_phase(k_full + ks, (j / KS) & 1, p.status, 0x409);  // complete: S came from this stage
+            uint8_t *k = smem + S::kKOff + ks * S::kStr + (32 * half + key) * 128 + (lane & 3) * 32;
 #pragma unroll
             for (int c = 0; c < kBlocks; ++c)
 #pragma unroll
@@ -273,8 +285,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           tc::fence_proxy_async_smem();
         }
       }
-      // dS of tile j - 2 was in this buffer; its dQ product was issued before S of this tile.
-      tc::tmem_st_32x32b_x16(lanes + kDsCol + (j & 1) * 32 + 16 * half, ds);
+      // dQ has read the dS of tile j - 2 in this buffer.
+      if (half == 0 && j >= 2 && !(ok = warp_wait(k_empty + (j - 2) % KS, ((j - 2) / KS) & 1, p.status, 0x40E))) break;
+      tc::tmem_st_32x32b_x16(lanes + kDsCol + set * 32 + 16 * half, ds);
       if (kBias && dbias) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -287,16 +300,18 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
               if (k + e < a.nk) reinterpret_cast<uint16_t *>(dbias)[k + e] = uint16_t(ds[4 * c + (e >> 1)] >> (16 * (e & 1)));
         }
       }
+      }
+      if (!ok) break;
       tc::tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(ds_full + (j & 1));
+      if (lane == 0) tc::mbar_arrive(ds_full + set);
     }
     if (ok && n > 0) ok = warp_wait(dq_full, 0, p.status, 0x40A);
     tc::tc_fence_after();
     if (ok) {
       Bf *dq = static_cast<Bf *>(p.x.dq) + ((int64_t(b) * a.nq + i) * a.heads + h) * a.d;
-      for (int c = half; c < (a.d + 15) / 16; c += 2) {
+      for (int c = set; c < (a.d + 15) / 16; c += 2) {
         uint32_t o[16];
         if (n > 0) {
           tc::tmem_ld_32x32b_x16(lanes + kDqCol + 16 * c, o);
@@ -328,15 +343,19 @@ template <int kBlocks, bool kBias, bool kLow> struct KShape {
   static constexpr int kRes = kRowsTc * 128 * kBlocks, kStr = kTileTc * 128 * kBlocks;
   static constexpr int kPer = kLow ? 3 : 2;  // streamed tiles: Q, dO, do - bf16(do)
   static constexpr int kB = kBias ? kTileTc * kRowsTc * 2 : 0;
-  static constexpr int kStages = kBlocks == 2 ? (kLow ? 2 : 3) : 3;
+  static constexpr int kStages = kBlocks == 1 ? (kBias ? 4 : 5) : kLow && kBias ? 2 : kLow || kBias ? 3 : 4;
   static constexpr int kStrOff = 2 * kRes;  // K, V
   static constexpr int kBiasOff = kStrOff + kStages * kPer * kStr;
   static constexpr int kStatOff = kBiasOff + kStages * kB;  // [stage]{reference, -log2 sum, base-2 offset, -delta}[64]
   static constexpr int kBarOff = kStatOff + kStages * 4 * kTileTc * 4 + kStages * 16;
   static constexpr int kBytes = kBarOff + 256 + 1024;
 };
-// TMEM columns: S^T, dP^T (64 each), two buffers of P^T and of dS^T (32 each), dV, dK.
-constexpr uint32_t kPtCol = 128, kDstCol = 192, kDvCol = 256, kDkCol = 384;
+// TMEM columns: two buffers of S^T and dP^T (64 each), of P^T and dS^T (32 each), dV, dK.  With wide
+// rows P^T and dS^T take the first columns of S^T and dP^T instead.
+template <int kBlocks> struct KCols {
+  static constexpr uint32_t pt = kBlocks == 1 ? 256 : kSCol, pt_step = kBlocks == 1 ? 32 : kPair;
+  static constexpr uint32_t ds = kBlocks == 1 ? 320 : kDpCol, dv = kBlocks == 1 ? 384 : 256, dk = dv + 64 * kBlocks;
+};
 
 template <int kBlocks, bool kBias, bool kLow>
 __global__ void __launch_bounds__(kThreadsTc, 1)
@@ -344,6 +363,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                    const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_bias, const BackTc p) {
   using S = KShape<kBlocks, kBias, kLow>;
+  using C = KCols<kBlocks>;
   constexpr int ST = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -353,10 +373,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t *st_empty = st_full + ST;     // [ST] dV and dK have read them
   uint64_t *stat_full = st_empty + ST;   // [ST] the rows' statistics are in shared memory
   uint64_t *stat_empty = stat_full + ST; // [ST] they (and the bias block) have been read
-  uint64_t *s_full = stat_empty + ST;    // S^T and dP^T in TMEM
-  uint64_t *s_free = s_full + 1;         // they are in registers
-  uint64_t *ps_full = s_free + 1;        // [2] P^T and dS^T in TMEM
-  uint64_t *d_full = ps_full + 2;        // every product is done
+  uint64_t *s_full = stat_empty + ST;    // [2] S^T and dP^T in TMEM
+  uint64_t *ps_full = s_full + 2;        // [2] P^T and dS^T in TMEM
+  uint64_t *pv_done = ps_full + 2;       // [2] dV has read P^T
+  uint64_t *d_full = pv_done + 2;        // every product is done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_full + 1);
   float *stats = reinterpret_cast<float *>(smem + S::kStatOff);
   int *lowest_flag = reinterpret_cast<int *>(stats + ST * 4 * kTileTc);  // [ST], 16 bytes apart
@@ -369,10 +389,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     tc::mbar_init(res_full, 1);
     for (int i = 0; i < ST; ++i) {
       tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1);
-      tc::mbar_init(stat_full + i, 1), tc::mbar_init(stat_empty + i, 8);
+      tc::mbar_init(stat_full + i, 1), tc::mbar_init(stat_empty + i, 4);
     }
-    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8), tc::mbar_init(d_full, 1);
-    tc::mbar_init(ps_full, 8), tc::mbar_init(ps_full + 1, 8);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(s_full + i, 2), tc::mbar_init(ps_full + i, 4), tc::mbar_init(pv_done + i, 1);
+    tc::mbar_init(d_full, 1);
     tc::fence_mbar_init();
   }
   if (warp == 1) {
@@ -410,98 +430,115 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
     }
   } else if (warp == 1) {
+    // ---------------- S^T ----------------
     if (lane == 0 && n > 0 && wait_phase(res_full, 0, p.status, 0x413)) {
       constexpr uint32_t idesc_s = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
-      const int steps = (a.d + 15) / 16;
-      const uint32_t idesc_d = tc::idesc_bf16(kRowsTc, 16 * steps, false, true);
-      const uint32_t base = smem_addr(smem);
-      auto product = [&](uint32_t col, uint32_t res, uint32_t str, bool add) {
-        for (int e = 0; e < steps; ++e)
-          tc::umma_f16_ss(tmem + col, desc_k(res + (e >> 2) * kRowsTc * 128 + (e & 3) * 32),
-                          desc_k(str + (e >> 2) * kTileTc * 128 + (e & 3) * 32), idesc_s, add || e != 0);
-      };
-      auto issue = [&](int u) {
-        const int s = u % ST;
-        if (!wait_phase(st_full + s, (u / ST) & 1, p.status, 0x414)) return false;
-        if (u > 0 && !wait_phase(s_free, (u - 1) & 1, p.status, 0x415)) return false;
+      const uint32_t base = low_k(smem_addr(smem));
+      for (int u = 0; u < n; ++u) {
+        const int s = u % ST, set = u & 1;
+        // The scores of this buffer are in registers (and what overwrote them has been read).
+        if (u >= 2 && !wait_phase((kBlocks == 1 ? ps_full : pv_done) + set, ((u - 2) >> 1) & 1, p.status, 0x415)) break;
+        if (!wait_phase(st_full + s, (u / ST) & 1, p.status, 0x414)) break;
         tc::tc_fence_after();
-        const uint32_t q = base + S::kStrOff + s * S::kPer * S::kStr;
-        product(kSCol, base, q, false);
-        product(kDpCol, base + S::kRes, q + S::kStr, false);
-        if (kLow) product(kDpCol, base + S::kRes, q + 2 * S::kStr, true);
-        tc::umma_commit(s_full);
-        return true;
-      };
-      bool ok = issue(0);
-      for (int u = 0; u < n && ok; ++u) {
-        if (u + 1 < n && !(ok = issue(u + 1))) break;
-        if (!(ok = wait_phase(ps_full + (u & 1), (u >> 1) & 1, p.status, 0x416))) break;
-        tc::tc_fence_after();
-        const uint32_t q = base + S::kStrOff + (u % ST) * S::kPer * S::kStr, d = q + S::kStr;
-#pragma unroll
-        for (int e = 0; e < kTileTc / 16; ++e)
-          tc::umma_f16_ts(tmem + kDvCol, tmem + kPtCol + (u & 1) * 32 + e * 8, tc::desc_sw128(d + e * 2048, kTileTc * 128),
-                          idesc_d, (u | e) != 0);
-        if (kLow)
-#pragma unroll
-          for (int e = 0; e < kTileTc / 16; ++e)
-            tc::umma_f16_ts(tmem + kDvCol, tmem + kPtCol + (u & 1) * 32 + e * 8,
-                            tc::desc_sw128(d + S::kStr + e * 2048, kTileTc * 128), idesc_d, true);
-#pragma unroll
-        for (int e = 0; e < kTileTc / 16; ++e)
-          tc::umma_f16_ts(tmem + kDkCol, tmem + kDstCol + (u & 1) * 32 + e * 8, tc::desc_sw128(q + e * 2048, kTileTc * 128),
-                          idesc_d, (u | e) != 0);
-        tc::umma_commit(st_empty + u % ST);
-        if (u + 1 == n) tc::umma_commit(d_full);
+        mma_rows_ss<kBlocks>(tmem + set * kPair + kSCol, base, kRowsTc * 128, base + ((S::kStrOff + s * S::kPer * S::kStr) >> 4),
+                             kTileTc * 128, idesc_s, false);
+        tc::umma_commit(s_full + set);
       }
     }
   } else if (warp == 2) {
-    // ---------------- statistics of the query rows, a tile at a time ----------------
-    for (int u = 0; u < n; ++u) {
-      const int s = u % ST, h = hk * a.group + u / q_tiles, i0 = u % q_tiles * kTileTc;
-      float m[2], nl[2], dl[2];
+    // ---------------- statistics of the query rows, a tile at a time, and dP^T ----------------
+    float m[2], nl[2], dl[2];
+    auto fetch = [&](int u) {
+      const int h = hk * a.group + u / q_tiles, i0 = u % q_tiles * kTileTc;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = i0 + lane + 32 * e;
         const int64_t at = (int64_t(b) * a.heads + h) * a.nq + i;
-        m[e] = i < a.nq ? row_max(a.lse[at]) : INFINITY;
-        nl[e] = i < a.nq ? -kLog2e * a.lse[a.lse_plane() + at] : 0.f;
-        dl[e] = i < a.nq ? -p.x.delta[at] : 0.f;
+        m[e] = i < a.nq ? a.lse[at] : -INFINITY;
+        nl[e] = i < a.nq ? a.lse[a.lse_plane() + at] : 0.f;
+        dl[e] = i < a.nq ? p.x.delta[at] : 0.f;
       }
-      if (u >= ST && !warp_wait(stat_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x417)) break;
+    };
+    constexpr uint32_t idesc_s = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
+    const uint32_t base = low_k(smem_addr(smem));
+    bool ok = n > 0 && warp_wait(res_full, 0, p.status, 0x41C);
+    if (ok) fetch(0);
+    for (int u = 0; u < n && ok; ++u) {
+      const int s = u % ST, set = u & 1;
+      if (u >= ST && !(ok = warp_wait(stat_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x417))) break;
       float *st = stats + s * 4 * kTileTc;
+      bool low = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = lane + 32 * e;
-        st[r] = m[e], st[kTileTc + r] = nl[e], st[3 * kTileTc + r] = dl[e];
-        st[2 * kTileTc + r] = m[e] == INFINITY ? -INFINITY : fmaf(-m[e], kLog2e, nl[e]);
+        const float top = row_max(m[e]), off = -kLog2e * nl[e];
+        st[r] = top, st[kTileTc + r] = off, st[3 * kTileTc + r] = -dl[e];
+        st[2 * kTileTc + r] = top == INFINITY ? -INFINITY : fmaf(-top, kLog2e, off);
+        low |= top < -1e37f;
       }
-      const bool lowest = __any_sync(0xffffffffu, m[0] < -1e37f || m[1] < -1e37f);
+      const bool lowest = __any_sync(0xffffffffu, low);
       if (lane == 0) lowest_flag[4 * s] = lowest;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(stat_full + s);
+      if (u + 1 < n) fetch(u + 1);
+      if (lane == 0) {
+        ok = u < 2 || (kBlocks == 1 ? wait_phase(ps_full + set, ((u - 2) >> 1) & 1, p.status, 0x41D)
+                                    : wait_phase(st_empty + (u - 2) % ST, ((u - 2) / ST) & 1, p.status, 0x41D));
+        ok = ok && wait_phase(st_full + s, (u / ST) & 1, p.status, 0x41E);
+        if (ok) {
+          tc::tc_fence_after();
+          const uint32_t d = base + ((S::kStrOff + s * S::kPer * S::kStr + S::kStr) >> 4);
+          mma_rows_ss<kBlocks>(tmem + set * kPair + kDpCol, base + (S::kRes >> 4), kRowsTc * 128, d, kTileTc * 128, idesc_s, false);
+          if (kLow)
+            mma_rows_ss<kBlocks>(tmem + set * kPair + kDpCol, base + (S::kRes >> 4), kRowsTc * 128, d + (S::kStr >> 4),
+                                 kTileTc * 128, idesc_s, true);
+          tc::umma_commit(s_full + set);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+  } else if (warp == 3) {
+    // ---------------- dV and dK ----------------
+    if (lane == 0) {
+      const uint32_t idesc_d = tc::idesc_bf16(kRowsTc, (a.d + 15) / 16 * 16, false, true);
+      const uint32_t base = low_mn(smem_addr(smem), kTileTc * 128);
+      for (int u = 0; u < n; ++u) {
+        const int s = u % ST, set = u & 1;
+        if (!wait_phase(ps_full + set, (u >> 1) & 1, p.status, 0x416) || !wait_phase(st_full + s, (u / ST) & 1, p.status, 0x41F))
+          break;
+        tc::tc_fence_after();
+        const uint32_t q = base + ((S::kStrOff + s * S::kPer * S::kStr) >> 4), d = q + (S::kStr >> 4);
+        const uint32_t pt = tmem + C::pt + set * C::pt_step, ds = tmem + C::ds + set * C::pt_step;
+        mma_cols_ts<kTileTc / 16>(tmem + C::dv, pt, d, idesc_d, u != 0);
+        if (kLow) mma_cols_ts<kTileTc / 16>(tmem + C::dv, pt, d + (S::kStr >> 4), idesc_d, true);
+        tc::umma_commit(pv_done + set);
+        mma_cols_ts<kTileTc / 16>(tmem + C::dk, ds, q, idesc_d, u != 0);
+        tc::umma_commit(st_empty + s);
+        if (u + 1 == n) tc::umma_commit(d_full);
+      }
     }
   } else if (warp >= 4) {
-    const int half = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
+    const int set = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, j = j0 + row;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
     const float mkv = mask_value(a, b, j);
     const bool out = mkv == -INFINITY;
     const uint64_t scale2 = dup2(a.scale), log2e2 = dup2(kLog2e), mk2 = dup2(out ? 0.f : mkv);
     const bool adds = __any_sync(0xffffffffu, !out && mkv != 0.f);
     bool ok = true;
-    for (int u = 0; u < n && ok; ++u) {
+    const uint32_t pair = lanes + set * kPair;
+    for (int u = set; u < n && ok; u += 2) {
       const int s = u % ST;
-      if (!(ok = warp_wait(s_full, u & 1, p.status, 0x418))) break;
+      if (!(ok = warp_wait(stat_full + s, (u / ST) & 1, p.status, 0x419) &&
+                 (!kBias || warp_wait(st_full + s, (u / ST) & 1, p.status, 0x41A)) &&
+                 warp_wait(s_full + set, (u >> 1) & 1, p.status, 0x418)))
+        break;
       tc::tc_fence_after();
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
       uint32_t sv[32], dv[32];
-      tc::tmem_ld_32x32b_x32(lanes + kSCol + 32 * half, sv);
-      tc::tmem_ld_32x32b_x32(lanes + kDpCol + 32 * half, dv);
-      ok = warp_wait(stat_full + s, (u / ST) & 1, p.status, 0x419) && (!kBias || warp_wait(st_full + s, (u / ST) & 1, p.status, 0x41A));
+      tc::tmem_ld_32x32b_x32(pair + kSCol + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(pair + kDpCol + 32 * half, dv);
       tc::tmem_ld_wait_regs(sv, dv);
-      if (!ok) break;
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(s_free);
       const float *st = stats + s * 4 * kTileTc + 32 * half;
       const bool lowest = lowest_flag[4 * s] != 0;
       // bias(q, key): 64-key block row / 64, row q of 128 bytes, 16-byte chunk (key / 8) ^ (q & 7).
@@ -531,26 +568,31 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         pt[e] = out ? 0u : pack_bf16x2(p0, p1);
         ds[e] = out ? 0u : pack_bf16x2(lo_f(g), hi_f(g));
       }
-      // The buffers' last products were issued before S^T of this tile, whose commit covers them.
-      tc::tmem_st_32x32b_x16(lanes + kPtCol + (u & 1) * 32 + 16 * half, pt);
-      tc::tmem_st_32x32b_x16(lanes + kDstCol + (u & 1) * 32 + 16 * half, ds);
+      // Wide rows: over columns that this half or the first one has read.  Else dV and dK have
+      // read what tile u - 2 left here.
+      if (kBlocks == 1 && half == 0 && u >= 2 && !(ok = warp_wait(st_empty + (u - 2) % ST, ((u - 2) / ST) & 1, p.status, 0x420)))
+        break;
+      tc::tmem_st_32x32b_x16(lanes + C::pt + set * C::pt_step + 16 * half, pt);
+      tc::tmem_st_32x32b_x16(lanes + C::ds + set * C::pt_step + 16 * half, ds);
+      }
+      if (!ok) break;
       tc::tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         tc::mbar_arrive(stat_empty + s);
-        tc::mbar_arrive(ps_full + (u & 1));
+        tc::mbar_arrive(ps_full + set);
       }
     }
     if (ok && n > 0) ok = warp_wait(d_full, 0, p.status, 0x41B);
     tc::tc_fence_after();
     if (ok) {
       const int64_t at = ((int64_t(b) * a.nk + j) * kv_heads + hk) * a.d;
-      for (int c = half; c < (a.d + 15) / 16; c += 2) {
+      for (int c = set; c < (a.d + 15) / 16; c += 2) {
         uint32_t gv[16], gk[16];
         if (n > 0) {
-          tc::tmem_ld_32x32b_x16(lanes + kDvCol + 16 * c, gv);
-          tc::tmem_ld_32x32b_x16(lanes + kDkCol + 16 * c, gk);
+          tc::tmem_ld_32x32b_x16(lanes + C::dv + 16 * c, gv);
+          tc::tmem_ld_32x32b_x16(lanes + C::dk + 16 * c, gk);
           tc::tmem_ld_wait();
         }
 #pragma unroll
@@ -650,17 +692,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
-      const int steps = (a.d + 15) / 16;
+      const uint32_t res = low_k(smem_addr(smem));
       for (int u = 0; u < n; ++u) {
         const int s = u & 1;
         if (!wait_phase(st_full + s, (u >> 1) & 1, p.status, 0x423)) break;
         if (u > 0 && !wait_phase(s_free, (u - 1) & 1, p.status, 0x424)) break;
         tc::tc_fence_after();
-        const uint32_t q = smem_addr(smem) + s * S::kStage, k = q + S::kPer * S::kRes;
-        for (int e = 0; e < steps; ++e) tc::umma_f16_ss(tmem, desc_k(q + e * 32), desc_k(k + e * 32), idesc, e != 0);
+        const uint32_t q = res + (s * S::kStage >> 4), k = q + (S::kPer * S::kRes >> 4);
+        mma_rows_ss<1>(tmem, q, 0, k, 0, idesc, false);
+#pragma unroll
         for (int t = 1; t < S::kPer; ++t)
-          for (int e = 0; e < steps; ++e)
-            tc::umma_f16_ss(tmem + 64, desc_k(q + t * S::kRes + e * 32), desc_k(k + S::kStr + e * 32), idesc, t > 1 || e != 0);
+          mma_rows_ss<1>(tmem + 64, q + (t * S::kRes >> 4), 0, k + (S::kStr >> 4), 0, idesc, t > 1);
         tc::umma_commit(s_full);
         tc::umma_commit(st_empty + s);
       }

@@ -161,16 +161,13 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       constexpr uint32_t idesc_s = tc::idesc_bf16(kBQ, kBK, false, false);
       const int steps = (a.d + 15) / 16;  // columns past d are zero
       const uint32_t idesc_pv = tc::idesc_bf16(kBQ, 16 * steps, false, true);
-      const uint32_t base = smem_addr(smem), q = base + t * S::kQ;
+      const uint32_t rows = low_k(smem_addr(smem)), cols = low_mn(smem_addr(smem), kBK * 128), q = rows + (t * S::kQ >> 4);
       auto issue_s = [&](int j) {
         const int s = j % KV;
         if (!wait_phase(kv_full + s, (j / KV) & 1, x.status, 0x304)) return false;
         if (j > 0 && !wait_phase(s_free + t, (j - 1) & 1, x.status, 0x305)) return false;
         tc::tc_fence_after();
-        const uint32_t k = base + S::kKvOff + s * 2 * S::kK;
-        for (int e = 0; e < steps; ++e)
-          tc::umma_f16_ss(tmem + t * 256, desc_k(q + (e >> 2) * kBQ * 128 + (e & 3) * 32),
-                          desc_k(k + (e >> 2) * kBK * 128 + (e & 3) * 32), idesc_s, e != 0);
+        mma_rows_ss<kBlocks>(tmem + t * 256, q, kBQ * 128, rows + ((S::kKvOff + s * 2 * S::kK) >> 4), kBK * 128, idesc_s, false);
         tc::umma_commit(s_full + t);
         return true;
       };
@@ -180,11 +177,8 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
         if (j + 1 < n_tiles && !(ok = issue_s(j + 1))) break;
         if (!(ok = wait_phase(p_full + t * 2 + buf, (j >> 1) & 1, x.status, 0x306))) break;
         tc::tc_fence_after();
-        const uint32_t v = base + S::kKvOff + s * 2 * S::kK + S::kK;
-#pragma unroll
-        for (int e = 0; e < kBK / 16; ++e)
-          tc::umma_f16_ts(tmem + t * 256 + S::kOCol, tmem + t * 256 + S::kPCol + buf * 32 + e * 8,
-                          tc::desc_sw128(v + e * 2048, kBK * 128), idesc_pv, (j | e) != 0);
+        mma_cols_ts<kBK / 16>(tmem + t * 256 + S::kOCol, tmem + t * 256 + S::kPCol + buf * 32,
+                              cols + ((S::kKvOff + s * 2 * S::kK + S::kK) >> 4), idesc_pv, j != 0);
         tc::umma_commit(pv_done + t * 2 + buf);
         tc::umma_commit(kv_empty + s);
         if (j + 1 == n_tiles) tc::umma_commit(o_full + t);

@@ -63,6 +63,34 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsign
   return __all_sync(0xffffffffu, wait_phase(bar, parity, status, code));
 }
 
+// The MMA issuers compute only the low words of descriptors (address, offset between blocks) and
+// unroll over the K steps: building 64-bit descriptors in a loop took 92 cycles per MMA of 64
+// columns, this 53, of which 48 are the operands' shared-memory reads.
+__device__ __forceinline__ uint32_t low_k(uint32_t saddr) { return uint32_t(desc_k(saddr)); }
+__device__ __forceinline__ uint32_t low_mn(uint32_t saddr, uint32_t block_bytes) {
+  return uint32_t(tc::desc_sw128(saddr, block_bytes));
+}
+__device__ __forceinline__ uint64_t with_low(uint32_t low) {
+  return uint64_t(low) | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// D (+)= A B^T over kBlocks * 64 columns: A and B rows of 128-byte swizzled 64-column blocks that are
+// a_block and b_block bytes apart, their descriptors' low words.  Columns past d are zero and
+// multiplied all the same: a test per step costs more than the steps.
+template <int kBlocks>
+__device__ __forceinline__ void mma_rows_ss(uint32_t d_tmem, uint32_t a, int a_block, uint32_t b, int b_block,
+                                            uint32_t idesc, bool add) {
+#pragma unroll
+  for (int e = 0; e < 4 * kBlocks; ++e)
+    tc::umma_f16_ss(d_tmem, with_low(a + (e >> 2) * (a_block >> 4) + (e & 3) * 2),
+                    with_low(b + (e >> 2) * (b_block >> 4) + (e & 3) * 2), idesc, add || e != 0);
+}
+// D (+)= A B over 16 kSteps rows of B: A 16-bit pairs in TMEM, B rows of 128 bytes, low_mn's word.
+template <int kSteps>
+__device__ __forceinline__ void mma_cols_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool add) {
+#pragma unroll
+  for (int e = 0; e < kSteps; ++e) tc::umma_f16_ts(d_tmem, a_tmem + e * 8, with_low(b + e * 128), idesc, add || e != 0);
+}
+
 __device__ __forceinline__ int n_words(int nk) { return (nk + 31) / 32; }
 // Bits of keys [32 w, 32 w + 32): left out by a keep mask, changed by an additive one, or past nk.
 __device__ __forceinline__ uint32_t mask_word(const Args &a, int b, int w) {
