@@ -253,14 +253,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = add2(y[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
       uint32_t ds[16];
+      if (lowest)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          y[e] = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
+      else
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = fma2(y[e], log2e2, c2);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        uint64_t z;
-        if (lowest)
-          z = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
-        else
-          z = fma2(y[e], log2e2, c2);
-        const uint64_t prob = pack2(__float_as_uint(fast_exp2(lo_f(z))), __float_as_uint(fast_exp2(hi_f(z))));
+        const uint64_t prob = pack2(__float_as_uint(fast_exp2(lo_f(y[e]))), __float_as_uint(fast_exp2(hi_f(y[e]))));
         const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
         ds[e] = pack_bf16x2(lo_f(g), hi_f(g));
       }
@@ -523,7 +525,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const float mkv = mask_value(a, b, j);
     const bool out = mkv == -INFINITY;
     const uint64_t scale2 = dup2(a.scale), log2e2 = dup2(kLog2e), mk2 = dup2(out ? 0.f : mkv);
-    const bool adds = __any_sync(0xffffffffu, !out && mkv != 0.f);
     bool ok = true;
     const uint32_t pair = lanes + set * kPair;
     for (int u = set; u < n && ok; u += 2) {
@@ -545,24 +546,28 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const uint8_t *bias = smem + S::kBiasOff + s * S::kB + (row >> 6) * kTileTc * 128 + 32 * half * 128 + (row & 7) * 2;
       const int chunk = (row & 63) >> 3;
       uint32_t pt[16], ds[16];
+      uint64_t z[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        uint64_t y;
         if constexpr (kBias) {
           const uint32_t b0 = *reinterpret_cast<const uint16_t *>(bias + (2 * e) * 128 + ((chunk ^ ((2 * e) & 7)) << 4));
           const uint32_t b1 = *reinterpret_cast<const uint16_t *>(bias + (2 * e + 1) * 128 + ((chunk ^ ((2 * e + 1) & 7)) << 4));
-          y = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(b0 << 16, b1 << 16));
+          z[e] = add2(fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(b0 << 16, b1 << 16)), mk2);
         } else {
-          y = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
+          z[e] = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, mk2);
         }
-        if (adds) y = add2(y, mk2);
-        uint64_t z;
-        if (lowest)
-          z = pack2(__float_as_uint(fmaf(lo_f(y) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
-                    __float_as_uint(fmaf(hi_f(y) - st[2 * e + 1], kLog2e, st[kTileTc + 2 * e + 1])));
-        else
-          z = fma2(y, log2e2, *reinterpret_cast<const uint64_t *>(st + 2 * kTileTc + 2 * e));
-        const float p0 = fast_exp2(lo_f(z)), p1 = fast_exp2(hi_f(z));
+      }
+      if (lowest)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
+                       __float_as_uint(fmaf(hi_f(z[e]) - st[2 * e + 1], kLog2e, st[kTileTc + 2 * e + 1])));
+      else
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = fma2(z[e], log2e2, *reinterpret_cast<const uint64_t *>(st + 2 * kTileTc + 2 * e));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p0 = fast_exp2(lo_f(z[e])), p1 = fast_exp2(hi_f(z[e]));
         const uint64_t prob = pack2(__float_as_uint(p0), __float_as_uint(p1));
         const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), *reinterpret_cast<const uint64_t *>(st + 3 * kTileTc + 2 * e)));
         pt[e] = out ? 0u : pack_bf16x2(p0, p1);
@@ -743,27 +748,37 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (lane == 0) tc::mbar_arrive(s_free);
       const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta);
       const uint32_t brow = smem_addr(smem + S::kBiasOff + (jt & 1) * S::kB) + row * 128;
+      uint64_t z[16];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const uint4 v = lds128(brow + (((4 * half + c) ^ (row & 7)) << 4));
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const int e = 4 * c + e4;
-          uint64_t y = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(w[e4] << 16, w[e4] & 0xffff0000u));
-          if (adds) y = add2(y, *reinterpret_cast<const uint64_t *>(mk + 2 * e));
-          uint64_t z;
-          if (lowest)
-            z = pack2(__float_as_uint(fmaf(lo_f(y) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y) - m, kLog2e, nl)));
-          else
-            z = fma2(y, log2e2, c2);
-          uint64_t g = mul2(pack2(__float_as_uint(fast_exp2(lo_f(z))), __float_as_uint(fast_exp2(hi_f(z)))),
-                            add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
-          const uint32_t out = cut >> (2 * e);
-          if (cut) g = pack2(out & 1 ? 0u : uint32_t(g), out & 2 ? 0u : uint32_t(g >> 32));
-          acc[e] = first ? g : add2(acc[e], g);
-        }
+        for (int e = 0; e < 4; ++e)
+          z[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
       }
+      if (adds)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = add2(z[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
+      if (lowest)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(z[e]) - m, kLog2e, nl)));
+      else
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = fma2(z[e], log2e2, c2);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        z[e] = mul2(pack2(__float_as_uint(fast_exp2(lo_f(z[e]))), __float_as_uint(fast_exp2(hi_f(z[e])))),
+                    add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
+      if (cut)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t out = cut >> (2 * e);
+          z[e] = pack2(out & 1 ? 0u : uint32_t(z[e]), out & 2 ? 0u : uint32_t(z[e] >> 32));
+        }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = first ? z[e] : add2(acc[e], z[e]);
       if ((u + 1) % a.share == 0) {
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(b_empty + (jt & 1));
