@@ -450,6 +450,205 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) bias_kernel
   }
 }
 
+// fp32 windows (17 to 32 queries, at most 128 keys, heads of their own): everything a (sample,
+// head) needs fits in shared memory, so one CTA makes all four gradients from one set of scores,
+// five products instead of the nine of the kernels above, and reads each tensor once.  Warp w
+// has query rows 16 (w & 1) and keys 32 (w / 2); P and dS go through shared memory to the keys'
+// products (16 keys per warp), dq is summed over the four key blocks.  The CTA walks the samples
+// that share a bias, dbias stays in its registers.
+constexpr int kWinThreads = 256, kWinRows = 32, kWinKeys = 128, kWinLd = kWinKeys + 4;
+
+template <int DP> constexpr size_t window_smem() {
+  return (2 * kWinRows * kLd<float, DP> + 2 * kWinKeys * kLd<float, DP> + kWinRows * kWinLd + kWinKeys + 3 * kWinRows) * 4;
+}
+static_assert(kWinKeys * kLd<float, 32> >= kWinRows * kWinLd, "P takes V's place");
+
+// acc[DP / 8][4] += A^T B over the kWinRows rows of A ([row][kWinLd], 16 columns from `a`) and B ([row][kLd]).
+// A step's rows are taken in the order 0, 2, 4, 6, 1, 3, 5, 7: without bank conflicts.
+template <int DP> __device__ __forceinline__ void mma_cols(float (&acc)[DP / 8][4], const float *a, const float *b, int lane) {
+  constexpr int ld = kLd<float, DP>;
+  const int g = lane >> 2, t = lane & 3;
+  const float *ap = a + 2 * t * kWinLd + g, *bp = b + 2 * t * ld + g;
+#pragma unroll
+  for (int n0 = 0; n0 < DP / 8; n0 += 4) {
+    float small[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) small[n][0] = small[n][1] = small[n][2] = small[n][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < kWinRows / 8; ++kk) {
+      uint32_t ah[4], al[4], bh[4][2], bl[4][2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split_tf32(ap[(kk * 8 + (e >> 1)) * kWinLd + (e & 1) * 8], ah[e], al[e]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) split_tf32(bp[(kk * 8 + e) * ld + (n0 + n) * 8], bh[n][e], bl[n][e]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) mma8(small[n], al, bh[n]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) mma8(acc[n0 + n], ah, bh[n]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) mma8(small[n], ah, bl[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n0 + n][e] += small[n][e];
+  }
+}
+
+template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kernel(const BackArgs x, int samples) {
+  constexpr int ld = kLd<float, DP>, ND = DP / 8, NT = 4;
+  const Args &a = x.a;
+  extern __shared__ float4 smem4[];
+  float *qs = reinterpret_cast<float *>(smem4), *dos = qs + kWinRows * ld, *ks = dos + kWinRows * ld, *vs = ks + kWinKeys * ld;
+  float *dss = vs + kWinKeys * ld, *mks = dss + kWinRows * kWinLd, *st = mks + kWinKeys;
+  float *ps = vs, *red = ks;  // once V, then K have been read
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = 16 * (warp & 1), c0 = 32 * (warp >> 1), key0 = 16 * warp;
+  const int h = int(blockIdx.x % a.heads), b0 = int(blockIdx.x / a.heads) * samples;
+  float *dbias = x.dbias ? static_cast<float *>(x.dbias) + (int64_t(b0 / a.share) * a.heads + h) * a.nq * x.dbias_ld : nullptr;
+  const float *bias = a.bias ? static_cast<const float *>(a.bias) + (b0 / a.share) * a.bias_sb + h * a.bias_sh : nullptr;
+  float sum[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
+  for (int b = b0; b < b0 + samples; ++b) {
+    const float *q = static_cast<const float *>(a.q.p) + b * a.q.sb + h * a.q.sh;
+    const float *k = static_cast<const float *>(a.k.p) + b * a.k.sb + h * a.k.sh;
+    const float *v = static_cast<const float *>(a.v.p) + b * a.v.sb + h * a.v.sh;
+    const float *dout = static_cast<const float *>(x.dout) + (int64_t(b) * a.nq * a.heads + h) * a.d;
+    load_rows<float, DP, kWinRows>(qs, q, a.q.si, 0, a.nq, a.d, tid, kWinThreads);
+    load_rows<float, DP, kWinRows>(dos, dout, int64_t(a.heads) * a.d, 0, a.nq, a.d, tid, kWinThreads);
+    load_rows<float, DP, kWinKeys>(ks, k, a.k.si, 0, a.nk, a.d, tid, kWinThreads);
+    load_rows<float, DP, kWinKeys>(vs, v, a.v.si, 0, a.nk, a.d, tid, kWinThreads);
+    cp_commit();
+    bool gone = false;
+    if (tid < kWinKeys) {
+      const float mk = mask_value(a, b, tid);
+      mks[tid] = mk;
+      gone = mk == -INFINITY;
+    } else if (tid < kWinKeys + kWinRows) {
+      const int i = tid - kWinKeys;
+      const int64_t at = (int64_t(b) * a.heads + h) * a.nq + i;
+      st[i] = i < a.nq ? row_max(a.lse[at]) : INFINITY;
+      st[kWinRows + i] = i < a.nq ? -kLog2e * a.lse[a.lse_plane() + at] : 0.f;
+      st[2 * kWinRows + i] = i < a.nq ? x.delta[at] : 0.f;
+    }
+    cp_wait_all();
+    if (__syncthreads_or(gone)) {
+      clear_left_out<float, DP, kWinKeys>(ks, mks, tid, kWinThreads);
+      clear_left_out<float, DP, kWinKeys>(vs, mks, tid, kWinThreads);
+      __syncthreads();
+    }
+    float s[NT][4], dp[NT][4], dq[ND][4];
+#pragma unroll
+    for (int n = 0; n < ND; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
+    if (c0 < a.nk) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = dp[n][e] = 0.f;
+      mma_rows<NT, DP>(s, qs + r0 * ld, ks + c0 * ld, lane);
+      mma_rows<NT, DP>(dp, dos + r0 * ld, vs + c0 * ld, lane);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = r0 + g + 8 * r;
+        const float m = st[i], nl = st[kWinRows + i], delta = st[2 * kWinRows + i];
+        const float *br = bias ? bias + int64_t(i) * a.bias_si + c0 + 2 * t : nullptr;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int j = c0 + n * 8 + 2 * t;
+          float2 bv = make_float2(0.f, 0.f);
+          if (br && i < a.nq) {
+            if (a.bias_vec && j + 1 < a.nk)
+              bv = *reinterpret_cast<const float2 *>(br + n * 8);
+            else
+              bv = make_float2(j < a.nk ? br[n * 8] : 0.f, j + 1 < a.nk ? br[n * 8 + 1] : 0.f);
+          }
+          const float2 mk = load2(mks + j);
+          grad_score(s[n][2 * r], dp[n][2 * r], a.scale, bv.x, mk.x, m, nl, delta);
+          grad_score(s[n][2 * r + 1], dp[n][2 * r + 1], a.scale, bv.y, mk.y, m, nl, delta);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[n][e] += dp[n][e];
+      mma_acc<NT, DP>(dq, dp, ks + c0 * ld, lane);
+    }
+    __syncthreads();
+    if (c0 < a.nk)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int at = (r0 + g + 8 * r) * kWinLd + c0 + n * 8 + 2 * t;
+          store2(ps + at, s[n][2 * r], s[n][2 * r + 1]);
+          store2(dss + at, dp[n][2 * r], dp[n][2 * r + 1]);
+        }
+    // dq of this key block, where K was.
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        store2(red + ((warp >> 1) * kWinRows + r0 + g + 8 * r) * ld + n * 8 + 2 * t, dq[n][2 * r], dq[n][2 * r + 1]);
+    __syncthreads();
+    if (key0 < a.nk) {
+      const int64_t at = ((int64_t(b) * a.nk + key0 + g) * a.heads + h) * a.d;
+      auto product = [&](const float *left, const float *right, void *to, float scale) {
+        float acc[ND][4];
+#pragma unroll
+        for (int n = 0; n < ND; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        mma_cols<DP>(acc, left + key0, right, lane);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (key0 + g + 8 * r < a.nk)
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+              if (n * 8 + 2 * t < a.d)
+                store2(static_cast<float *>(to) + at + int64_t(8 * r) * a.heads * a.d + n * 8 + 2 * t, scale * acc[n][2 * r],
+                       scale * acc[n][2 * r + 1]);
+      };
+      product(ps, dos, x.dv, 1.f);
+      product(dss, qs, x.dk, a.scale);
+    }
+    for (int u = tid; u < kWinRows * (DP / 4); u += kWinThreads) {
+      const int i = u / (DP / 4), c = u % (DP / 4) * 4;
+      if (i >= a.nq || c >= a.d) continue;
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 y = *reinterpret_cast<const float4 *>(red + (e * kWinRows + i) * ld + c);
+        w.x += y.x, w.y += y.y, w.z += y.z, w.w += y.w;
+      }
+      *reinterpret_cast<float4 *>(static_cast<float *>(x.dq) + ((int64_t(b) * a.nq + i) * a.heads + h) * a.d + c) =
+          make_float4(w.x * a.scale, w.y * a.scale, w.z * a.scale, w.w * a.scale);
+    }
+    __syncthreads();
+  }
+  if (dbias && c0 < a.nk)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (r0 + g + 8 * r < a.nq)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          store_bias(dbias + (r0 + g + 8 * r) * x.dbias_ld, c0 + n * 8 + 2 * t, a.nk, sum[n][2 * r], sum[n][2 * r + 1]);
+}
+
+// *taken where the windows' kernel has run.  Below one CTA per SM the kernels above have the GPU's other SMs to win.
+template <int DP> int launch_window(const BackArgs &x, cudaStream_t stream, bool *taken) {
+  const Args &a = x.a;
+  const int samples = x.dbias ? a.share : 1;
+  const int64_t ctas = int64_t(a.batch / samples) * a.heads;
+  *taken = a.group == 1 && a.nq > 16 && a.nq <= kWinRows && a.nk > 32 && a.nk <= kWinKeys && ctas >= num_sms();
+  if (!*taken) return BL_OK;
+  BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention_backward: too many windows");
+  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(window_kernel<DP>), 232448));
+  window_kernel<DP><<<unsigned(ctas), kWinThreads, window_smem<DP>(), stream>>>(x, samples);
+  BL_LAUNCH_CHECK();
+  return BL_OK;
+}
+
 template <typename T, int DP> int launch(const BackArgs &x, cudaStream_t stream) {
   const Args &a = x.a;
   const bool biased = a.bias != nullptr;
@@ -458,6 +657,10 @@ template <typename T, int DP> int launch(const BackArgs &x, cudaStream_t stream)
   rows_kernel<T><<<unsigned((rows_total + 31) / 32), 256, 0, stream>>>(x, rows_total);
   BL_LAUNCH_CHECK();
   bool taken = false;
+  if constexpr (sizeof(T) == 4 && DP <= 64) {
+    if (int rc = launch_window<DP>(x, stream, &taken)) return rc;
+    if (taken) return BL_OK;
+  }
   if (sizeof(T) == 2)
     if (int rc = keys_tc(x, stream, &taken)) return rc;
   if (a.nk > 0 && !taken) {

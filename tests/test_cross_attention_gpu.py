@@ -85,6 +85,42 @@ def test_values_and_gradients(case, dtype):
     check(run(to_cuda(x), backward=False), *reference(**x))
 
 
+WINDOWS = [
+    # b, nq, nk, h, hk, d, share, gate, mask: enough (bias, head) pairs to fill the GPU with windows
+    (192, 32, 128, 4, 4, 32, 2, True, "add"),
+    (90, 17, 33, 3, 3, 24, 1, False, "keep"),
+    (128, 31, 127, 2, 2, 64, 0, True, "tail"),
+    (160, 20, 96, 4, 4, 40, 2, True, "fraction"),
+    (80, 32, 65, 4, 4, 8, 1, True, "none"),
+    (60, 16, 128, 4, 2, 32, 1, True, "keep"),
+]
+
+
+@pytest.mark.parametrize("case", WINDOWS)
+def test_windows(case):
+    test_values_and_gradients(case, torch.float32)
+
+
+def test_windows_left_out_keys_hold_anything():
+    """NaN and infinities of left-out keys reach nothing, rows without keys and of lowest values follow the definition."""
+    x = inputs(160, 24, 100, 4, 4, 32, torch.float32, 2, True, "keep")
+    x["mask"][1] = False
+    x["mask"][2, :64] = False
+    x["mask"][2, 64] = True
+    x["bias"][3, :, 0] = -math.inf
+    x["bias"][4, :, 1] = torch.finfo(torch.float32).min
+    clean = {n: t.clone() if isinstance(t, torch.Tensor) else t for n, t in x.items()}
+    bad = ~x["mask"]
+    x["k"][bad], x["v"][bad] = math.nan, math.inf
+    both = ~(x["mask"][0::2] | x["mask"][1::2])
+    x["bias"] = torch.where(both[:, None, None], math.nan, x["bias"])
+    actual, want = run(to_cuda(x)), run(to_cuda(clean))
+    for n in actual:
+        assert torch.equal(actual[n], want[n]), n
+    assert not actual["dq"][1].any() and not actual["dk"][bad.cuda()].any() and not actual["dv"][bad.cuda()].any()
+    check(actual, *reference(**clean))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nq", [2, 90, 260])
 def test_left_out_keys_hold_anything(dtype, nq):
