@@ -18,7 +18,7 @@ template <typename T, int DP> struct FlashSmem {
   static constexpr int bn = kBN<T, DP>, ld = kLd<T, DP>;
   static size_t bytes(int rows, bool bias) {
     return size_t(rows) * ld * sizeof(T) + 2 * (2 * bn * ld * sizeof(T) + bn * 4) +
-           (bias ? 2 * size_t(rows) * (bn + 8) * sizeof(T) : 0);
+           (bias && sizeof(T) == 2 ? 2 * size_t(rows) * (bn + 8) * sizeof(T) : 0);
   }
 };
 
@@ -42,7 +42,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
   auto load = [&](int j, int buf) {
     load_rows<T, DP, BN>(ks + buf * BN * ld, k, a.k.si, j * BN, a.nk, a.d, tid, threads);
     load_rows<T, DP, BN>(vs + buf * BN * ld, v, a.v.si, j * BN, a.nk, a.d, tid, threads);
-    if (bias) load_bias<T, BN>(bs + buf * rows * (BN + 8), bias, a, i0, rows, j * BN, tid, threads);
+    if (sizeof(T) == 2 && bias) load_bias<T, BN>(bs + buf * rows * (BN + 8), bias, a, i0, rows, j * BN, tid, threads);
     cp_commit();
   };
   for (int u = tid; u < rows * (DP / Type<T>::kVec); u += threads) {
@@ -77,8 +77,24 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
 #pragma unroll
   for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
+  // fp32 bias: straight into registers (the staged blocks left room for 6 CTAs of 64 threads per SM, not 9).
+  float2 bv[sizeof(T) == 4 ? NT : 1][2];
   for (int j = 0; j < n_tiles; ++j) {
     const int buf = j & 1;
+    if constexpr (sizeof(T) == 4)
+      if (bias) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = i0 + warp * 16 + g + 8 * r;
+          const float *br = bias + int64_t(i) * a.bias_si + j * BN + 2 * t;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int left = i < a.nq ? a.nk - j * BN - n * 8 - 2 * t : 0;
+            bv[n][r] = a.bias_vec && left > 1 ? *reinterpret_cast<const float2 *>(br + n * 8)
+                                              : make_float2(left > 0 ? br[n * 8] : 0.f, left > 1 ? br[n * 8 + 1] : 0.f);
+          }
+        }
+      }
     if (j + 1 < n_tiles) {
       load(j + 1, buf ^ 1);
       cp_wait<1>();
@@ -106,7 +122,11 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float2 b0 = make_float2(0.f, 0.f), b1 = b0;
-        if (bias) b0 = load2(br + n * 8), b1 = load2(br + 8 * (BN + 8) + n * 8);
+        if constexpr (sizeof(T) == 4) {
+          if (bias) b0 = bv[n][0], b1 = bv[n][1];
+        } else {
+          if (bias) b0 = load2(br + n * 8), b1 = load2(br + 8 * (BN + 8) + n * 8);
+        }
         s[n][0] = fmaf(s[n][0], a.scale, b0.x), s[n][1] = fmaf(s[n][1], a.scale, b0.y);
         s[n][2] = fmaf(s[n][2], a.scale, b1.x), s[n][3] = fmaf(s[n][3], a.scale, b1.y);
         if (masked) {
