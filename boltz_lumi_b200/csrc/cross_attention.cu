@@ -88,11 +88,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
           const int i = i0 + warp * 16 + g + 8 * r;
           const float *br = bias + int64_t(i) * a.bias_si + j * BN + 2 * t;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int left = i < a.nq ? a.nk - j * BN - n * 8 - 2 * t : 0;
-            bv[n][r] = a.bias_vec && left > 1 ? *reinterpret_cast<const float2 *>(br + n * 8)
-                                              : make_float2(left > 0 ? br[n * 8] : 0.f, left > 1 ? br[n * 8 + 1] : 0.f);
-          }
+          for (int n = 0; n < NT; ++n) bv[n][r] = bias_pair(a, br + n * 8, i < a.nq ? a.nk - j * BN - n * 8 - 2 * t : 0);
         }
       }
     if (j + 1 < n_tiles) {

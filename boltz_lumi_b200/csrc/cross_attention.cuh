@@ -107,6 +107,12 @@ __device__ __forceinline__ void load_bias(T *dst, const T *bias, const Args &a, 
   }
 }
 
+// Two neighbouring elements of an fp32 bias row from an even column, `left` of the row at hand (the others 0).
+__device__ __forceinline__ float2 bias_pair(const Args &a, const float *p, int left) {
+  if (a.bias_vec && left > 1) return *reinterpret_cast<const float2 *>(p);
+  return make_float2(left > 0 ? p[0] : 0.f, left > 1 ? p[1] : 0.f);
+}
+
 // mk of key j (see above); keys past nk are left out.
 __device__ __forceinline__ float mask_value(const Args &a, int b, int j) {
   if (j >= a.nk) return -INFINITY;

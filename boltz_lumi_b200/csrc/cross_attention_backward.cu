@@ -91,7 +91,7 @@ constexpr int kKeys = 64;
 
 template <typename T, int DP> size_t keys_smem(bool bias, bool low) {
   constexpr int ld = kLd<T, DP>, BQ = kTile<T, DP>;
-  return (2 * kKeys * ld + (low ? 6 : 4) * BQ * ld) * sizeof(T) + 6 * BQ * 4 + (bias ? 2 * BQ * (kKeys + 8) * sizeof(T) : 0);
+  return (2 * kKeys * ld + (low ? 6 : 4) * BQ * ld) * sizeof(T) + 6 * BQ * 4 + (bias && sizeof(T) == 2 ? 2 * BQ * (kKeys + 8) * sizeof(T) : 0);
 }
 
 template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel(const BackArgs x, int tiles) {
@@ -133,7 +133,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
       cp4(lg + buf * BQ + tid, a.lse + a.lse_plane() + at + (ok ? i0 + tid : 0), ok);
       cp4(del + buf * BQ + tid, x.delta + at + (ok ? i0 + tid : 0), ok);
     }
-    if (a.bias) {
+    if (sizeof(T) == 2 && a.bias) {
       const T *bias = static_cast<const T *>(a.bias) + (b / a.share) * a.bias_sb + h * a.bias_sh;
       load_bias<T, kKeys>(bs + buf * BQ * (kKeys + 8), bias, a, i0, BQ, j0, tid, kThreads);
     }
@@ -146,8 +146,20 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
 #pragma unroll
     for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
 
+  // fp32 bias: straight into registers (see flash_kernel).
+  float bv[sizeof(T) == 4 ? NT : 1][4];
   for (int u = 0; u < steps; ++u) {
     const int buf = u & 1;
+    if constexpr (sizeof(T) == 4)
+      if (a.bias) {
+        const int h = hk * a.group + u / q_tiles, i0 = u % q_tiles * BQ + 2 * t, j = j0 + warp * 16 + g;
+        const T *br = static_cast<const T *>(a.bias) + (b / a.share) * a.bias_sb + h * a.bias_sh + i0 * a.bias_si + j;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            bv[n][e] = i0 + n * 8 + (e & 1) < a.nq && j + (e >> 1) * 8 < a.nk ? br[(n * 8 + (e & 1)) * a.bias_si + (e >> 1) * 8] : 0.f;
+      }
     if (u + 1 < steps) {
       load(u + 1, buf ^ 1);
       cp_wait<1>();
@@ -171,16 +183,21 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
         const float2 lv = load2(ls + buf * BQ + n * 8 + 2 * t), dl = load2(del + buf * BQ + n * 8 + 2 * t);
         const float2 ll = load2(lg + buf * BQ + n * 8 + 2 * t);
         const float m0 = row_max(lv.x), m1 = row_max(lv.y), n0 = -kLog2e * ll.x, n1 = -kLog2e * ll.y;
-        float bv[4] = {0.f, 0.f, 0.f, 0.f};
+        float bq[4] = {0.f, 0.f, 0.f, 0.f};
         if (a.bias) {
-          const T *p = bp + n * 8 * (kKeys + 8);
-          bv[0] = load_as_float(p), bv[1] = load_as_float(p + kKeys + 8);
-          bv[2] = load_as_float(p + 8), bv[3] = load_as_float(p + kKeys + 16);
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bq[e] = bv[n][e];
+          } else {
+            const T *p = bp + n * 8 * (kKeys + 8);
+            bq[0] = load_as_float(p), bq[1] = load_as_float(p + kKeys + 8);
+            bq[2] = load_as_float(p + 8), bq[3] = load_as_float(p + kKeys + 16);
+          }
         }
-        grad_score(s[n][0], dp[n][0], a.scale, bv[0], mk[0], m0, n0, dl.x);
-        grad_score(s[n][1], dp[n][1], a.scale, bv[1], mk[0], m1, n1, dl.y);
-        grad_score(s[n][2], dp[n][2], a.scale, bv[2], mk[1], m0, n0, dl.x);
-        grad_score(s[n][3], dp[n][3], a.scale, bv[3], mk[1], m1, n1, dl.y);
+        grad_score(s[n][0], dp[n][0], a.scale, bq[0], mk[0], m0, n0, dl.x);
+        grad_score(s[n][1], dp[n][1], a.scale, bq[1], mk[0], m1, n1, dl.y);
+        grad_score(s[n][2], dp[n][2], a.scale, bq[2], mk[1], m0, n0, dl.x);
+        grad_score(s[n][3], dp[n][3], a.scale, bq[3], mk[1], m1, n1, dl.y);
       }
       if (x.dlow) mma_acc<NT, DP>(dv, s, dls + buf * BQ * ld, lane);
       mma_acc<NT, DP>(dv, s, dt, lane);
@@ -206,7 +223,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
 
 template <typename T, int DP> size_t queries_smem(int rows, bool bias, bool low) {
   constexpr int ld = kLd<T, DP>, BN = kTile<T, DP>;
-  return ((low ? 3 : 2) * size_t(rows) * ld + 4 * BN * ld) * sizeof(T) + 2 * BN * 4 + (bias ? 2 * size_t(rows) * (BN + 8) * sizeof(T) : 0);
+  return ((low ? 3 : 2) * size_t(rows) * ld + 4 * BN * ld) * sizeof(T) + 2 * BN * 4 + (bias && sizeof(T) == 2 ? 2 * size_t(rows) * (BN + 8) * sizeof(T) : 0);
 }
 
 // ds of two neighbouring keys of one row into the bias gradient's row.
@@ -239,7 +256,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
   auto load = [&](int j, int buf) {
     load_rows<T, DP, BN>(ks + buf * BN * ld, k, a.k.si, j * BN, a.nk, a.d, tid, threads);
     load_rows<T, DP, BN>(vs + buf * BN * ld, v, a.v.si, j * BN, a.nk, a.d, tid, threads);
-    if (bias) load_bias<T, BN>(bs + buf * rows * (BN + 8), bias, a, i0, rows, j * BN, tid, threads);
+    if (sizeof(T) == 2 && bias) load_bias<T, BN>(bs + buf * rows * (BN + 8), bias, a, i0, rows, j * BN, tid, threads);
     cp_commit();
   };
   constexpr int kChunks = DP / Type<T>::kVec;
@@ -285,8 +302,19 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
 
+  float2 bv[sizeof(T) == 4 ? NT : 1][2];  // fp32 bias (see flash_kernel)
   for (int j = 0; j < n_tiles; ++j) {
     const int buf = j & 1;
+    if constexpr (sizeof(T) == 4)
+      if (bias) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = i0 + warp * 16 + g + 8 * r;
+          const float *br = bias + int64_t(i) * a.bias_si + j * BN + 2 * t;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) bv[n][r] = bias_pair(a, br + n * 8, i < a.nq ? a.nk - j * BN - n * 8 - 2 * t : 0);
+        }
+      }
     if (j + 1 < n_tiles) {
       load(j + 1, buf ^ 1);
       cp_wait<1>();
@@ -315,7 +343,11 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float2 b0 = make_float2(0.f, 0.f), b1 = b0, m2 = b0;
-        if (bias) b0 = load2(br + n * 8), b1 = load2(br + 8 * (BN + 8) + n * 8);
+        if constexpr (sizeof(T) == 4) {
+          if (bias) b0 = bv[n][0], b1 = bv[n][1];
+        } else {
+          if (bias) b0 = load2(br + n * 8), b1 = load2(br + 8 * (BN + 8) + n * 8);
+        }
         if (masked) m2 = load2(mk + n * 8 + 2 * t);
         grad_score(s[n][0], dp[n][0], a.scale, b0.x, m2.x, m[0], nl[0], delta[0]);
         grad_score(s[n][1], dp[n][1], a.scale, b0.y, m2.y, m[0], nl[0], delta[0]);
@@ -455,7 +487,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) bias_kernel
 // five products instead of the nine of the kernels above, and reads each tensor once.  Warp w
 // has query rows 16 (w & 1) and keys 32 (w / 2); P and dS go through shared memory to the keys'
 // products (16 keys per warp), dq is summed over the four key blocks.  The CTA walks the samples
-// that share a bias, dbias stays in its registers.
+// that share a bias, dbias stays in its registers.  96 biases x 4 samples of 32 x 128, 4 heads of 32:
+// 76 us (150 with the kernels above); bound by the split products' issue and latency, not by bytes
+// (floor 17 us).
 constexpr int kWinThreads = 256, kWinRows = 32, kWinKeys = 128, kWinLd = kWinKeys + 4;
 
 template <int DP> constexpr size_t window_smem() {
@@ -558,13 +592,7 @@ template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kerne
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int j = c0 + n * 8 + 2 * t;
-          float2 bv = make_float2(0.f, 0.f);
-          if (br && i < a.nq) {
-            if (a.bias_vec && j + 1 < a.nk)
-              bv = *reinterpret_cast<const float2 *>(br + n * 8);
-            else
-              bv = make_float2(j < a.nk ? br[n * 8] : 0.f, j + 1 < a.nk ? br[n * 8 + 1] : 0.f);
-          }
+          const float2 bv = br ? bias_pair(a, br + n * 8, i < a.nq ? a.nk - j : 0) : make_float2(0.f, 0.f);
           const float2 mk = load2(mks + j);
           grad_score(s[n][2 * r], dp[n][2 * r], a.scale, bv.x, mk.x, m, nl, delta);
           grad_score(s[n][2 * r + 1], dp[n][2 * r + 1], a.scale, bv.y, mk.y, m, nl, delta);
@@ -635,12 +663,15 @@ template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kerne
           store_bias(dbias + (r0 + g + 8 * r) * x.dbias_ld, c0 + n * 8 + 2 * t, a.nk, sum[n][2 * r], sum[n][2 * r + 1]);
 }
 
-// *taken where the windows' kernel has run.  Below one CTA per SM the kernels above have the GPU's other SMs to win.
+// *taken where the windows' kernel has run.  At 32 x 128 x 4 heads it takes 13 us against 23 of the kernels above for
+// 4 biases of one sample, 35 against 41 for 16 biases of 4, but a CTA that walks many samples alone is slower (107
+// against 60 us for 1 bias of 16).  Below 17 queries or 33 keys half of its warps idle (43 against 39 us at 16 x 33).
 template <int DP> int launch_window(const BackArgs &x, cudaStream_t stream, bool *taken) {
   const Args &a = x.a;
   const int samples = x.dbias ? a.share : 1;
   const int64_t ctas = int64_t(a.batch / samples) * a.heads;
-  *taken = a.group == 1 && a.nq > 16 && a.nq <= kWinRows && a.nk > 32 && a.nk <= kWinKeys && ctas >= num_sms();
+  *taken = a.group == 1 && a.nq > 16 && a.nq <= kWinRows && a.nk > 32 && a.nk <= kWinKeys &&
+           (samples <= 4 || ctas >= 2 * num_sms());
   if (!*taken) return BL_OK;
   BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention_backward: too many windows");
   BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(window_kernel<DP>), 232448));
