@@ -626,13 +626,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 }
 
 // Gradient of a bias that several samples share: one CTA = 128 query rows of one (bias, head) over a
-// range of key tiles; for each tile the samples' Q, dO, K and V stream through a two-stage ring and the
+// range of key tiles; for each tile the samples' Q, dO, K and V stream through a three-stage ring and the
 // threads add up dS in registers.  d <= 64 (two 64-column blocks would leave one stage).
 template <bool kLow> struct BShape {
   static constexpr int kRes = kRowsTc * 128, kStr = kTileTc * 128, kPer = kLow ? 3 : 2;
   static constexpr int kStage = kPer * kRes + 2 * kStr;  // Q, dO, do - bf16(do), K, V
   static constexpr int kB = kRowsTc * kTileTc * 2;
-  static constexpr int kBiasOff = 2 * kStage, kMaskOff = kBiasOff + 2 * kB, kBarOff = kMaskOff + 8 * 32 * 4;
+  static constexpr int kStages = 3, kBiasOff = kStages * kStage, kMaskOff = kBiasOff + 2 * kB, kBarOff = kMaskOff + 8 * 32 * 4;
   static constexpr int kBytes = kBarOff + 256 + 1024;
 };
 
@@ -646,10 +646,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
-  uint64_t *st_full = bars, *st_empty = bars + 2;   // [2] a sample's tiles landed; its products are done
-  uint64_t *b_full = bars + 4, *b_empty = bars + 6; // [2] bias block landed; it has been read
-  uint64_t *s_full = bars + 8, *s_free = bars + 9;  // S and dP in TMEM; in registers
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10);
+  constexpr int ST = S::kStages;
+  uint64_t *st_full = bars, *st_empty = bars + ST;    // [ST] a sample's tiles landed; its products are done
+  uint64_t *b_full = st_empty + ST, *b_empty = b_full + 2;  // [2] bias block landed; it has been read
+  uint64_t *s_full = b_empty + 2, *s_free = s_full + 2;     // [2] S and dP in TMEM; in registers
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_free + 2);
   const Args &a = p.x.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int64_t at = blockIdx.x;
@@ -662,13 +663,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   const int t0 = int(int64_t(range) * key_tiles / ranges), t1 = int(int64_t(range + 1) * key_tiles / ranges);
   const int n = (t1 - t0) * a.share;  // (key tile, sample) steps
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i)
-      tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 1), tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 8);
-    tc::mbar_init(s_full, 1), tc::mbar_init(s_free, 8);
+    for (int i = 0; i < ST; ++i) tc::mbar_init(st_full + i, 1), tc::mbar_init(st_empty + i, 2);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(b_full + i, 1), tc::mbar_init(b_empty + i, 8);
+      tc::mbar_init(s_full + i, 2), tc::mbar_init(s_free + i, 8);
+    }
     tc::fence_mbar_init();
   }
   if (warp == 1) {
-    tc::tmem_alloc(tmem_slot, 128);
+    tc::tmem_alloc(tmem_slot, 256);
     tc::tmem_relinquish();
   }
   tc::tc_fence_before();
@@ -678,8 +681,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   if (warp == 0) {
     if (lane == 0)
       for (int u = 0; u < n; ++u) {
-        const int s = u & 1, jt = u / a.share, b = bb * a.share + u % a.share, j0 = (t0 + jt) * kTileTc;
-        if (u >= 2 && !wait_phase(st_empty + s, ((u >> 1) & 1) ^ 1u, p.status, 0x421)) break;
+        const int s = u % ST, jt = u / a.share, b = bb * a.share + u % a.share, j0 = (t0 + jt) * kTileTc;
+        if (u >= ST && !wait_phase(st_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x421)) break;
         uint8_t *st = smem + s * S::kStage;
         tc::mbar_arrive_expect_tx(st_full + s, S::kStage);
         tma_load_4d(st, &map_q, st_full + s, 0, q0, h, b);
@@ -694,21 +697,25 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           tma_load_4d(smem + S::kBiasOff + bs * S::kB, &map_bias, b_full + bs, j0, q0, h, bb);
         }
       }
-  } else if (warp == 1) {
+  } else if (warp < 3) {
+    // ---------------- S (warp 1) and dP (warp 2) ----------------
     if (lane == 0) {
       constexpr uint32_t idesc = tc::idesc_bf16(kRowsTc, kTileTc, false, false);
-      const uint32_t res = low_k(smem_addr(smem));
+      const uint32_t base = low_k(smem_addr(smem));
       for (int u = 0; u < n; ++u) {
-        const int s = u & 1;
-        if (!wait_phase(st_full + s, (u >> 1) & 1, p.status, 0x423)) break;
-        if (u > 0 && !wait_phase(s_free, (u - 1) & 1, p.status, 0x424)) break;
+        const int s = u % ST, buf = u & 1;
+        if (!wait_phase(st_full + s, (u / ST) & 1, p.status, 0x423)) break;
+        if (u >= 2 && !wait_phase(s_free + buf, ((u - 2) >> 1) & 1, p.status, 0x424)) break;
         tc::tc_fence_after();
-        const uint32_t q = res + (s * S::kStage >> 4), k = q + (S::kPer * S::kRes >> 4);
-        mma_rows_ss<1>(tmem, q, 0, k, 0, idesc, false);
+        const uint32_t q = base + (s * S::kStage >> 4), k = q + (S::kPer * S::kRes >> 4);
+        if (warp == 1) {
+          mma_rows_ss<1>(tmem + buf * kPair + kSCol, q, 0, k, 0, idesc, false);
+        } else {
 #pragma unroll
-        for (int t = 1; t < S::kPer; ++t)
-          mma_rows_ss<1>(tmem + 64, q + (t * S::kRes >> 4), 0, k + (S::kStr >> 4), 0, idesc, t > 1);
-        tc::umma_commit(s_full);
+          for (int t = 1; t < S::kPer; ++t)
+            mma_rows_ss<1>(tmem + buf * kPair + kDpCol, q + (t * S::kRes >> 4), 0, k + (S::kStr >> 4), 0, idesc, t > 1);
+        }
+        tc::umma_commit(s_full + buf);
         tc::umma_commit(st_empty + s);
       }
     }
@@ -718,15 +725,22 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     float *mk = reinterpret_cast<float *>(smem + S::kMaskOff) + (warp - 4) * 32;
     const uint64_t scale2 = dup2(a.scale), log2e2 = dup2(kLog2e);
     uint64_t acc[16];
-    for (int u = 0; u < n; ++u) {
-      const int jt = u / a.share, first = u % a.share == 0, b = bb * a.share + u % a.share;
-      const int k0 = (t0 + jt) * kTileTc + 32 * half;
-      float m = INFINITY, nl = 0.f, delta = 0.f;
+    // A step's statistics and mask values are fetched a step ahead.
+    float m, nl, delta, mv;
+    auto fetch = [&](int u) {
+      const int b = bb * a.share + u % a.share;
+      m = -INFINITY, nl = delta = 0.f;
       if (i < a.nq) {
         const int64_t r = (int64_t(b) * a.heads + h) * a.nq + i;
-        m = row_max(a.lse[r]), nl = -kLog2e * a.lse[a.lse_plane() + r], delta = p.x.delta[r];
+        m = a.lse[r], nl = a.lse[a.lse_plane() + r], delta = p.x.delta[r];
       }
-      const float mv = mask_value(a, b, k0 + lane);
+      mv = mask_value(a, b, (t0 + u / a.share) * kTileTc + 32 * half + lane);
+    };
+    if (n > 0) fetch(0);
+    for (int u = 0; u < n; ++u) {
+      const int jt = u / a.share, first = u % a.share == 0, buf = u & 1;
+      const int k0 = (t0 + jt) * kTileTc + 32 * half;
+      m = row_max(m), nl *= -kLog2e;
       const bool adds = __any_sync(0xffffffffu, mv != 0.f && mv != -INFINITY);
       const uint32_t cut = __ballot_sync(0xffffffffu, mv == -INFINITY);
       if (adds) {
@@ -735,18 +749,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         __syncwarp();
       }
       const bool lowest = __any_sync(0xffffffffu, m < -1e37f);
-      if (!warp_wait(s_full, u & 1, p.status, 0x425)) break;
+      const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta);
+      const float m_now = m, nl_now = nl;
+      if (u + 1 < n) fetch(u + 1);
+      if (!warp_wait(s_full + buf, (u >> 1) & 1, p.status, 0x425)) break;
       tc::tc_fence_after();
       uint32_t sv[32], dv[32];
-      tc::tmem_ld_32x32b_x32(lanes + 32 * half, sv);
-      tc::tmem_ld_32x32b_x32(lanes + 64 + 32 * half, dv);
+      tc::tmem_ld_32x32b_x32(lanes + buf * kPair + kSCol + 32 * half, sv);
+      tc::tmem_ld_32x32b_x32(lanes + buf * kPair + kDpCol + 32 * half, dv);
       const bool ok = !first || warp_wait(b_full + (jt & 1), (jt >> 1) & 1, p.status, 0x426);
       tc::tmem_ld_wait_regs(sv, dv);
       if (!ok) break;
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(s_free);
-      const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta);
+      if (lane == 0) tc::mbar_arrive(s_free + buf);
       const uint32_t brow = smem_addr(smem + S::kBiasOff + (jt & 1) * S::kB) + row * 128;
       uint64_t z[16];
 #pragma unroll
@@ -763,7 +779,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (lowest)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(z[e]) - m, kLog2e, nl)));
+          z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - m_now, kLog2e, nl_now)), __float_as_uint(fmaf(hi_f(z[e]) - m_now, kLog2e, nl_now)));
       else
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[e] = fma2(z[e], log2e2, c2);
@@ -805,7 +821,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 128);
+    tc::tmem_dealloc(tmem, 256);
   }
 }
 
