@@ -228,17 +228,6 @@ template <typename T, int DP> struct Step {
   static constexpr int bytes = q_bytes + (ring_bytes > part_bytes ? ring_bytes : part_bytes);
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float peer(const float *local, uint32_t rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(local)), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(32 * Step<T, DP>::warps) step_kernel(const Args a, int split) {
   using S = Step<T, DP>;

@@ -14,7 +14,10 @@
 // What bounds it: one exponential per score (16 per clock and SM) and, with a bias,
 // the bias bytes through L2; the products are a third of that.  Two query tiles per
 // CTA halve the K / V bytes that each score costs; with few tiles one per CTA
-// spreads them over more SMs.
+// spreads them over more SMs, and a cluster of CTAs divides the keys of one tile
+// and joins its parts through distributed shared memory (one launch, fixed order).
+#include <array>
+
 #include "cross_attention_tc.cuh"
 
 namespace bl {
@@ -48,9 +51,62 @@ template <int kTiles, int kBlocks, bool kBias> struct Shape {  // kBlocks: 64-co
 
 struct TcArgs {
   Args a;
-  int q_tiles;  // CTAs per (sample, head)
+  int q_tiles;  // CTAs (clusters) per (sample, head)
+  int split;    // CTAs of a cluster that divide the keys
   unsigned int *status;
 };
+
+// Joins the parts of a cluster's CTAs (in the order of their keys): a thread has one row and every
+// split-th group of four columns.
+__device__ __forceinline__ void merge_rows(const Args &a, const void *part, const void *stat, int split, int rank, int row,
+                                           int q0, int h, int b) {
+  const int i = q0 + row;
+  if (i >= a.nq) return;
+  const float *st = static_cast<const float *>(stat);
+  float weight[8], top = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    weight[e] = e < split ? peer(st + row, uint32_t(e)) : -INFINITY;
+    top = fmaxf(top, weight[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    weight[e] = weight[e] == -INFINITY ? 0.f : fast_exp2((weight[e] - top) * kLog2e);
+    if (e < split) l = fmaf(weight[e], peer(st + kBQ + row, uint32_t(e)), l);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  using T = __nv_bfloat16;
+  const int64_t at = ((int64_t(b) * a.nq + i) * a.heads + h) * a.d;
+  const T *gate = a.gate.p ? static_cast<const T *>(a.gate.p) + b * a.gate.sb + int64_t(i) * a.gate.si + h * a.gate.sh : nullptr;
+  for (int c = rank; 4 * c < a.d; c += split) {
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < split) {
+        const float4 v = peer4(static_cast<const float4 *>(part) + c * kBQ + row, uint32_t(e));
+        o[0] = fmaf(weight[e], v.x, o[0]), o[1] = fmaf(weight[e], v.y, o[1]);
+        o[2] = fmaf(weight[e], v.z, o[2]), o[3] = fmaf(weight[e], v.w, o[3]);
+      }
+    uint2 g = make_uint2(0u, 0u);
+    if (gate) g = *reinterpret_cast<const uint2 *>(gate + 4 * c);
+    const float gv[4] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] *= inv;
+      if (gate) o[e] *= 1.f / (1.f + expf(-gv[e]));
+    }
+    const uint2 hi = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at + 4 * c) = hi;
+    if (a.low)
+      *reinterpret_cast<uint2 *>(static_cast<T *>(a.low) + at + 4 * c) =
+          make_uint2(pack_bf16x2(o[0] - bf16_lo(hi.x), o[1] - bf16_hi(hi.x)), pack_bf16x2(o[2] - bf16_lo(hi.y), o[3] - bf16_hi(hi.y)));
+  }
+  if (a.lse && rank == 0) {
+    float *to = a.lse + (int64_t(b) * a.heads + h) * a.nq + i;
+    to[0] = l == 0.f ? -INFINITY : top;
+    to[a.lse_plane()] = l == 0.f ? 0.f : logf(l);
+  }
+}
 
 template <int kTiles, int kBlocks, bool kBias>
 __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTiles == 1 ? 2 : 1)
@@ -78,7 +134,8 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
   const Args &a = x.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int tile, h, b;
-  decode_cta(a, blockIdx.x, x.q_tiles, a.heads, tile, h, b);
+  const int split = kTiles == 1 ? x.split : 1, rank = split > 1 ? int(blockIdx.x) % split : 0;
+  decode_cta(a, blockIdx.x / split, x.q_tiles, a.heads, tile, h, b);
   const int q0 = tile * kTiles * kBQ, hk = h / a.group, bb = b / a.share;
   const int live = a.nq - q0 > kBQ ? kTiles : 1;  // query tiles with rows
 
@@ -121,7 +178,9 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       __syncthreads();
     }
   }
-  const int n_tiles = (keys + kBK - 1) / kBK;
+  // Key tiles [lo, lo + n_tiles).
+  const int all_tiles = (keys + kBK - 1) / kBK, lo = int(int64_t(rank) * all_tiles / split);
+  const int n_tiles = int(int64_t(rank + 1) * all_tiles / split) - lo;
 
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kFew));
   if (warp == 0) {
@@ -140,16 +199,16 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
         if (j >= KV && !(ok = wait_phase(kv_empty + s, ((j / KV) & 1) ^ 1u, x.status, 0x301))) break;
         uint8_t *st = smem + S::kKvOff + s * 2 * S::kK;
         tc::mbar_arrive_expect_tx(kv_full + s, 2 * S::kK);
-        for (int c = 0; c < kBlocks; ++c) tma_load_4d(st + c * kBK * 128, &map_k, kv_full + s, 64 * c, j * kBK, hk, b);
+        for (int c = 0; c < kBlocks; ++c) tma_load_4d(st + c * kBK * 128, &map_k, kv_full + s, 64 * c, (lo + j) * kBK, hk, b);
         for (int c = 0; c < kBlocks; ++c)
-          tma_load_4d(st + S::kK + c * kBK * 128, &map_v, kv_full + s, 64 * c, j * kBK, hk, b);
+          tma_load_4d(st + S::kK + c * kBK * 128, &map_v, kv_full + s, 64 * c, (lo + j) * kBK, hk, b);
         if constexpr (kBias) {
           const int bs = j % BS;
           for (int t = 0; t < live; ++t) {
             uint64_t *full = b_full + t * BS + bs;
             if (j >= BS && !(ok = wait_phase(b_empty + t * BS + bs, ((j / BS) & 1) ^ 1u, x.status, 0x302))) break;
             tc::mbar_arrive_expect_tx(full, S::kB);
-            tma_load_4d(smem + S::kBiasOff + (t * BS + bs) * S::kB, &map_bias, full, j * kBK, q0 + t * kBQ, h, bb);
+            tma_load_4d(smem + S::kBiasOff + (t * BS + bs) * S::kB, &map_bias, full, (lo + j) * kBK, q0 + t * kBQ, h, bb);
           }
         }
       }
@@ -207,25 +266,25 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
     };
     if (ok && n_tiles > 0) fetch(0);
     for (int j = 0; j < n_tiles && ok; ++j) {
-      const int buf = j & 1, bs = j % BS;
+      const int buf = j & 1, bs = j % BS, k0 = (lo + j) * kBK;
       // Keys of this tile that the mask touches, and keys past nk.
       uint32_t cut[2] = {0u, 0u};
       if (a.mask_kind == kMaskNone) {
-        const int left = a.nk - j * kBK;
+        const int left = a.nk - k0;
         if (left < kBK) cut[0] = left < 32 ? ~0u << left : 0u, cut[1] = left <= 32 ? ~0u : ~0u << (left - 32);
       } else if (use_bits) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(bits + 2 * j);
+        const uint2 w = *reinterpret_cast<const uint2 *>(bits + 2 * (lo + j));
         cut[0] = w.x, cut[1] = w.y;
       } else {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          cut[e] = __ballot_sync(0xffffffffu, mask_value(a, b, j * kBK + 32 * e + lane) != 0.f);
+          cut[e] = __ballot_sync(0xffffffffu, mask_value(a, b, k0 + 32 * e + lane) != 0.f);
       }
       const bool masked = (cut[0] | cut[1]) != 0;
       if (masked && a.mask_kind == kMaskAdd) {
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 2; ++e) mk[lane + 32 * e] = mask_value(a, b, j * kBK + 32 * e + lane);
+        for (int e = 0; e < 2; ++e) mk[lane + 32 * e] = mask_value(a, b, k0 + 32 * e + lane);
         __syncwarp();
       }
       if constexpr (kBias) {
@@ -363,7 +422,25 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       const T *gate = a.gate.p ? static_cast<const T *>(a.gate.p) + b * a.gate.sb + int64_t(i) * a.gate.si + h * a.gate.sh
                                : nullptr;
       T *out = static_cast<T *>(a.out) + at, *low = a.low ? static_cast<T *>(a.low) + at : nullptr;
-      if (ok) {
+      if (ok && kTiles == 1 && split > 1) {
+        // This CTA's part of the row, for the cluster: O where K and V were, [4 columns][row].
+        float4 *part = reinterpret_cast<float4 *>(smem + S::kKvOff);
+        float *stat = reinterpret_cast<float *>(smem + S::kMaskOff);
+        for (int c = 0; c < d16; ++c) {
+          uint32_t o[16];
+          if (n_tiles > 0) {
+            tc::tmem_ld_32x32b_x16(o_col + 16 * c, o);
+            tc::tmem_ld_wait();
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            part[(4 * c + e) * kBQ + row] =
+                n_tiles > 0 ? make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                          __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]))
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        stat[row] = l == 0.f ? -INFINITY : m, stat[kBQ + row] = l;
+      } else if (ok) {
         for (int c = 0; c < d16; ++c) {
           uint32_t o[16];
           if (n_tiles > 0) {
@@ -393,7 +470,7 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
             if (low) *reinterpret_cast<uint4 *>(low + c0) = make_uint4(lv[0], lv[1], lv[2], lv[3]);
           }
         }
-        if (a.lse && i < a.nq) {
+        if (a.lse && i < a.nq) {  // (a cluster's rows: merge_rows)
           float *st = a.lse + (int64_t(b) * a.heads + h) * a.nq + i;
           st[0] = l == 0.f ? -INFINITY : m;
           st[a.lse_plane()] = l == 0.f ? 0.f : logf(l);
@@ -401,12 +478,43 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       }
     }
   }
+  if (kTiles == 1 && split > 1) {
+    __syncwarp();
+    cluster_barrier();
+    if (warp >= 4) merge_rows(a, smem + S::kKvOff, smem + S::kMaskOff, split, rank, tid - 128, q0, h, b);
+    __syncwarp();
+    cluster_barrier();  // until every part has been read
+  }
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, S::kTmem);
   }
+}
+
+// Clusters of s CTAs that the device holds at once.
+template <int kTiles, int kBlocks, bool kBias> int active_clusters(int s) {
+  using S = Shape<kTiles, kBlocks, kBias>;
+  static const std::array<int, 9> table = [] {
+    std::array<int, 9> t{};
+    for (int e = 1; e <= 8; ++e) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = unsigned(e), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(unsigned(e)), config.blockDim = dim3(S::kThreads), config.dynamicSmemBytes = S::kBytes;
+      config.attrs = attr, config.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, flash_tc_kernel<kTiles, kBlocks, kBias>, &config) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = num_sms() / e;
+      }
+      t[e] = n < 1 ? 1 : n;
+    }
+    return t;
+  }();
+  return table[s];
 }
 
 template <int kTiles, int kBlocks, bool kBias>
@@ -422,7 +530,26 @@ int launch_tc(const Args &a, const CUtensorMap (&maps)[4], cudaStream_t stream) 
   BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention: too many query tiles");
   auto kernel = flash_tc_kernel<kTiles, kBlocks, kBias>;
   BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(kernel), S::kBytes));
-  kernel<<<unsigned(ctas), S::kThreads, S::kBytes, stream>>>(maps[0], maps[1], maps[2], maps[3], x);
+  x.split = 1;
+  if (kTiles == 1) {
+    // Few CTAs: a cluster divides the keys, by the waves that it takes (128 queries, 8 heads: 33 -> 12 us at
+    // 1024 keys, 164 -> 29 us at 8192; 2 x 16 x 384 x 1734: 46 -> 39 us).
+    const int64_t work = (a.nk + kBK - 1) / kBK;
+    double best = 0.;
+    for (int e = 1; e <= 8 && (e == 1 || e <= work); ++e) {
+      const int64_t held = active_clusters<kTiles, kBlocks, kBias>(e), waves = (ctas + held - 1) / held;
+      const double cost = double(waves) / e + 0.02 * (e > 1);
+      if (e == 1 || cost < best) best = cost, x.split = e;
+    }
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(ctas * x.split)), config.blockDim = dim3(S::kThreads);
+  config.dynamicSmemBytes = S::kBytes, config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(x.split), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  config.attrs = attr, config.numAttrs = x.split > 1 ? 1 : 0;
+  BL_CUDA(cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], x));
   BL_LAUNCH_CHECK();
   return BL_OK;
 }

@@ -121,6 +121,40 @@ def test_windows_left_out_keys_hold_anything():
     check(actual, *reference(**clean))
 
 
+LONG = [
+    # few query tiles over many keys: the keys are divided
+    (1, 70, 1500, 2, 1, 128, 0, True, "keep"),
+    (2, 100, 2000, 2, 2, 32, 2, True, "add"),
+    (1, 257, 4099, 1, 1, 64, 1, False, "tail"),
+    (1, 128, 256, 3, 3, 96, 1, True, "fraction"),
+    (3, 90, 777, 1, 1, 40, 3, True, "none"),
+]
+
+
+@pytest.mark.parametrize("case", LONG)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_keys(case, dtype):
+    test_values_and_gradients(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [48, 128])
+def test_long_keys_left_out(dtype, d):
+    """Whole parts of the keys left out, a sample with one key, one without, rows of -inf and of lowest values."""
+    x = inputs(4, 100, 2050, 2, 2, d, dtype, 2, True, "keep")
+    x["mask"][0, :1300] = False
+    x["mask"][1, 600:] = False
+    x["mask"][2] = False
+    x["mask"][2, 2049] = True
+    x["mask"][3] = False
+    x["bias"][0, :, 0] = -math.inf
+    x["bias"][0, :, 1] = torch.finfo(dtype).min
+    x["bias"][0, :, 2, :1900] = -math.inf
+    actual = run(to_cuda(x))
+    assert not actual["out"][3].any() and (actual["lse"][0, 3] == -math.inf).all()
+    check(actual, *reference(**x))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nq", [2, 90, 260])
 def test_left_out_keys_hold_anything(dtype, nq):
