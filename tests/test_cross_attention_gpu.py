@@ -155,6 +155,40 @@ def test_long_keys_left_out(dtype, d):
     check(actual, *reference(**x))
 
 
+@pytest.mark.parametrize("d", range(8, 129, 8))
+def test_head_dims(d):
+    test_values_and_gradients((2, 70, 80, 2, 1, d, 2, d % 16 == 0, "keep"), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,nk", [(3, 50), (24, 100), (130, 200)])
+def test_scales(dtype, nq, nk):
+    """A negative scale is that of the negated queries; scale 0 leaves the bias alone."""
+    x = inputs(2, nq, nk, 2, 2, 32, dtype, 2, True, "keep")
+    value, bound = reference(**{**x, "q": -x["q"]}, scale=0.3)
+    value["dq"] = -value["dq"]
+    check(run(to_cuda(dict(x, scale=-0.3))), value, bound)
+    actual = run(to_cuda(dict(x, scale=0.0)))
+    assert not actual["dq"].any() and not actual["dk"].any()
+    check(actual, *reference(**x, scale=0.0))
+
+
+@pytest.mark.parametrize("mask", ["none", "keep", "add"])
+def test_more_keys_than_mask_bits(mask):
+    test_values_and_gradients((2, 70, 65601, 1, 1, 16, 2, True, mask), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_unaligned_bias_of_long_rows(dtype):
+    x = inputs(2, 140, 333, 2, 1, 48, dtype, 1, True, "fraction")
+    value, bound = reference(**x)
+    wide = torch.zeros(2, 2, 140, 335, dtype=dtype)
+    wide[..., 1:334] = x["bias"]
+    given = to_cuda(x)
+    given["bias"] = wide.cuda()[..., 1:334]
+    check(run(given), value, bound)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nq", [2, 90, 260])
 def test_left_out_keys_hold_anything(dtype, nq):

@@ -209,6 +209,35 @@ def test_bias_gradient(case, dtype, padded):
     assert torch.equal(out, kernels.relative_position_bias_backward(dyc, *where, num_buckets=buckets))
 
 
+@pytest.mark.parametrize("nk", [68, 70])
+def test_wide_positions_and_groups(nk):
+    """Positions and groups past 32 bits, in some samples and columns: offsets clip and groups differ in 64 bits."""
+    from boltz_lumi_b200 import kernels
+
+    g = torch.Generator().manual_seed(nk)
+    b, h, nq, buckets, distance = 3, 5, 37, 9, 6
+    table = torch.randn(buckets, h, generator=g)
+    lut = torch.randint(0, buckets, (2 * distance + 1,), generator=g, dtype=torch.int32)
+    q_pos, k_pos = torch.randint(-9, 9, (b, nq), generator=g), torch.randint(-9, 9, (b, nk), generator=g)
+    q_pos[1] += 2 ** 40
+    k_pos[1] += 2 ** 40  # far from zero, near one another
+    k_pos[2, ::7] += 2 ** 33
+    q_pos[2, ::5] += 2 ** 33
+    q_pos[0, 3], k_pos[0, 5] = 2 ** 62, -2 ** 61
+    q_group, k_group = torch.randint(0, 2, (b, nq), generator=g), torch.randint(0, 2, (b, nk), generator=g)
+    q_group[0, ::3] += 2 ** 32  # equal to another group in the low word
+    k_group[2, ::4] += 2 ** 32
+    k_group[0, 10] = 2 ** 32
+    for groups in ((None, None), (q_group, k_group)):
+        args = (table, q_pos, k_pos, lut, *groups)
+        u = bias_reference(*args)
+        assert torch.equal(kernels.relative_position_bias(*to_cuda(*args)).cpu(), table[u].permute(0, 3, 1, 2))
+        dy = torch.randint(-8, 9, (b, h, nq, nk), generator=g).float()  # exact sums
+        expected = torch.einsum("bhij,biju->uh", dy.double(), one_hot(u, buckets))
+        out = kernels.relative_position_bias_backward(dy.cuda(), *to_cuda(*args[1:]), num_buckets=buckets)
+        assert torch.equal(out.cpu().double(), expected)
+
+
 def test_bad_bucket_entries_count_as_last():
     """Entries of the bucket table outside the table never index past it."""
     from boltz_lumi_b200 import kernels
