@@ -22,7 +22,50 @@ template <typename T, int DP> struct FlashSmem {
   }
 };
 
-template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kernel(const Args a, int tiles) {
+template <int DP> constexpr int kPartLd = DP + 4;
+
+// Joins the parts of a cluster's CTAs in the order of their keys: a thread takes four columns of a row at a time.
+template <typename T, int DP>
+__device__ __forceinline__ void join_parts(const Args &a, const float *part, const float *stat, int rows, int split, int rank,
+                                           int i0, int h, int b) {
+  for (int u = rank * blockDim.x + threadIdx.x; u < rows * (DP / 4); u += split * blockDim.x) {
+    const int row = u / (DP / 4), c = u % (DP / 4) * 4, i = i0 + row;
+    if (i >= a.nq || c >= a.d) continue;
+    float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < split; ++e) top = fmaxf(top, peer(stat + row, uint32_t(e)));
+    for (int e = 0; e < split; ++e) {
+      const float m = peer(stat + row, uint32_t(e));
+      if (m == -INFINITY) continue;
+      const float weight = fast_exp2((m - top) * kLog2e);
+      l = fmaf(weight, peer(stat + rows + row, uint32_t(e)), l);
+      const float4 v = peer4(reinterpret_cast<const float4 *>(part + row * kPartLd<DP> + c), uint32_t(e));
+      x[0] = fmaf(weight, v.x, x[0]), x[1] = fmaf(weight, v.y, x[1]);
+      x[2] = fmaf(weight, v.z, x[2]), x[3] = fmaf(weight, v.w, x[3]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t at = ((int64_t(b) * a.nq + i) * a.heads + h) * a.d + c;
+    const T *gr = a.gate.p ? static_cast<const T *>(a.gate.p) + b * a.gate.sb + i * a.gate.si + h * a.gate.sh + c : nullptr;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] *= inv;
+      if (gr) x[e] *= 1.f / (1.f + expf(-load_as_float(gr + e)));
+    }
+    store4(static_cast<T *>(a.out) + at, x);
+    if constexpr (sizeof(T) == 2)
+      if (a.low) {
+        const float y[4] = {x[0] - bf16r(x[0]), x[1] - bf16r(x[1]), x[2] - bf16r(x[2]), x[3] - bf16r(x[3])};
+        store4(static_cast<T *>(a.low) + at, y);
+      }
+    if (a.lse && c == 0) {
+      float *st = a.lse + (int64_t(b) * a.heads + h) * a.nq + i;
+      st[0] = l == 0.f ? -INFINITY : top;
+      st[a.lse_plane()] = l == 0.f ? 0.f : logf(l);
+    }
+  }
+}
+
+// kSplit: as a cluster of `split` CTAs.  (A variant of its own: its registers cost the other 5 to 10 %.)
+template <typename T, int DP, bool kSplit> __global__ void __launch_bounds__(128) flash_kernel(const Args a, int tiles, int clusters) {
   constexpr int BN = kBN<T, DP>, NT = BN / 8, ld = kLd<T, DP>, ND = DP / 8;
   extern __shared__ float4 smem4[];
   const int threads = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -32,7 +75,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
   float *mks = reinterpret_cast<float *>(vs + 2 * BN * ld);
   T *bs = reinterpret_cast<T *>(mks + 2 * BN);
   int tile, h, b;
-  decode_cta(a, blockIdx.x, tiles, a.heads, tile, h, b);
+  const int split = kSplit ? clusters : 1, rank = kSplit ? int(blockIdx.x) % split : 0;
+  decode_cta(a, blockIdx.x / split, tiles, a.heads, tile, h, b);
   const int i0 = tile * rows, hk = h / a.group;
   const T *q = static_cast<const T *>(a.q.p) + b * a.q.sb + h * a.q.sh;
   const T *k = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -50,8 +94,10 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
     const bool ok = i0 + r < a.nq && c < a.d;
     cp16(qs + r * ld + c, ok ? q + int64_t(i0 + r) * a.q.si + c : q, ok ? 16 : 0);
   }
-  const int n_tiles = (a.nk + BN - 1) / BN;
-  if (n_tiles > 0) load(0, 0);
+  // Key tiles [first, n_tiles).
+  const int all_tiles = (a.nk + BN - 1) / BN, first = int(int64_t(rank) * all_tiles / split);
+  const int n_tiles = int(int64_t(rank + 1) * all_tiles / split);
+  if (n_tiles > first) load(first, 0);
   // mk of a tile: read into registers a tile ahead, put into shared memory after that tile's products.
   float mv[2];
   bool odd = false;
@@ -68,7 +114,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
       if (tid + e * threads < BN) mks[buf * BN + tid + e * threads] = mv[e];
     odd = mv[0] != 0.f || mv[1] != 0.f;
   };
-  get_mask(0);
+  get_mask(first);
   put_mask(0);
 
   const int g = lane >> 2, t = lane & 3;
@@ -79,8 +125,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
 
   // fp32 bias: straight into registers (the staged blocks left room for 6 CTAs of 64 threads per SM, not 9).
   float2 bv[sizeof(T) == 4 ? NT : 1][2];
-  for (int j = 0; j < n_tiles; ++j) {
-    const int buf = j & 1;
+  for (int j = first; j < n_tiles; ++j) {
+    const int buf = (j - first) & 1;
     if constexpr (sizeof(T) == 4)
       if (bias) {
 #pragma unroll
@@ -167,6 +213,24 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) flash_kerne
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  if constexpr (kSplit) {  // the cluster's parts, through shared memory
+    float *part = reinterpret_cast<float *>(smem4), *stat = part + rows * kPartLd<DP>;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = warp * 16 + g + 8 * r;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) store2(part + row * kPartLd<DP> + n * 8 + 2 * t, o[n][2 * r], o[n][2 * r + 1]);
+      if (t == 0) stat[row] = l[r] == 0.f ? -INFINITY : m[r], stat[rows + row] = l[r];
+    }
+    cluster_barrier();
+    join_parts<T, DP>(a, part, stat, rows, split, rank, i0, h, b);
+    cluster_barrier();  // until every part has been read
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
     const int i = i0 + warp * 16 + g + 8 * r;
     if (i >= a.nq) continue;
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
@@ -198,8 +262,11 @@ template <typename T, int DP> int launch_flash(const Args &a, cudaStream_t strea
   const int64_t tiles = (a.nq + rows - 1) / rows, ctas = tiles * a.heads * a.batch;
   BL_REQUIRE(ctas < (int64_t(1) << 31), "bl_cross_attention: too many query tiles");
   const size_t smem = FlashSmem<T, DP>::bytes(rows, a.bias != nullptr);
-  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(flash_kernel<T, DP>), 232448));
-  flash_kernel<T, DP><<<unsigned(ctas), 32 * warps, smem, stream>>>(a, int(tiles));
+  // Few CTAs: a cluster divides the keys.
+  const int split = key_split(ctas, (a.nk + kBN<T, DP> - 1) / kBN<T, DP>);
+  auto kernel = split > 1 ? flash_kernel<T, DP, true> : flash_kernel<T, DP, false>;
+  BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(kernel), 232448));
+  BL_CUDA(launch_clusters(kernel, ctas, split, 32 * warps, smem, stream, a, int(tiles), split));
   BL_LAUNCH_CHECK();
   return BL_OK;
 }

@@ -327,6 +327,29 @@ __device__ __forceinline__ void clear_left_out(T *rows, const float *mk, int tid
           make_uint4(0u, 0u, 0u, 0u);
 }
 
+// CTAs of a cluster that divide `tiles` key tiles, two or more each, where `ctas` clusters leave SMs without
+// two CTAs (128 threads or fewer each).
+inline int key_split(int64_t ctas, int64_t tiles) {
+  const int64_t room = ctas > 0 ? 2 * int64_t(num_sms()) / ctas : 1, most = room < tiles / 2 ? room : tiles / 2;
+  return most < 1 ? 1 : most > 8 ? 8 : int(most);
+}
+template <typename K, typename... A>
+cudaError_t launch_clusters(K kernel, int64_t ctas, int split, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(ctas * split)), config.blockDim = dim3(unsigned(threads));
+  config.dynamicSmemBytes = smem, config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(split), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  config.attrs = attr, config.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+// Four fp32 values to a row of the type.
+__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&v)[4]) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
 // cross_attention.cu
 Args make_args(const bl_cross_attention_args *x);
 int check(const char *name, const Args &a, int64_t kv_heads, int dtype);

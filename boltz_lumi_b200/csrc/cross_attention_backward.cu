@@ -234,7 +234,8 @@ template <typename T> __device__ __forceinline__ void store_bias(T *row, int j, 
     store_from_float(row + j, x);
 }
 
-template <typename T, int DP> __global__ void __launch_bounds__(128) queries_kernel(const BackArgs x, int tiles) {
+// kSplit: see flash_kernel.
+template <typename T, int DP, bool kSplit> __global__ void __launch_bounds__(128) queries_kernel(const BackArgs x, int tiles, int clusters) {
   constexpr int BN = kTile<T, DP>, NT = BN / 8, ld = kLd<T, DP>, ND = DP / 8;
   const Args &a = x.a;
   extern __shared__ float4 smem4[];
@@ -245,7 +246,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
   float *mks = reinterpret_cast<float *>(vs + 2 * BN * ld);
   T *bs = reinterpret_cast<T *>(mks + 2 * BN);
   int tile, h, b;
-  decode_cta(a, blockIdx.x, tiles, a.heads, tile, h, b);
+  const int split = kSplit ? clusters : 1, rank = kSplit ? int(blockIdx.x) % split : 0;
+  decode_cta(a, blockIdx.x / split, tiles, a.heads, tile, h, b);
   const int i0 = tile * rows, hk = h / a.group;
   const T *q = static_cast<const T *>(a.q.p) + b * a.q.sb + h * a.q.sh;
   const T *k = static_cast<const T *>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -270,8 +272,10 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
       cp16(dls + r * ld + c, ok ? low + int64_t(i0 + r) * a.heads * a.d + c : low, ok ? 16 : 0);
     }
   }
-  const int n_tiles = (a.nk + BN - 1) / BN;
-  if (n_tiles > 0) load(0, 0);
+  // Key tiles [first, n_tiles).
+  const int all_tiles = (a.nk + BN - 1) / BN, first = int(int64_t(rank) * all_tiles / split);
+  const int n_tiles = int(int64_t(rank + 1) * all_tiles / split);
+  if (n_tiles > first) load(first, 0);
   float m[2], nl[2], delta[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -296,15 +300,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
       if (tid + e * threads < BN) mks[buf * BN + tid + e * threads] = mv[e];
     odd = mv[0] != 0.f || mv[1] != 0.f;
   };
-  get_mask(0);
+  get_mask(first);
   put_mask(0);
   float dq[ND][4];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
 
   float2 bv[sizeof(T) == 4 ? NT : 1][2];  // fp32 bias (see flash_kernel)
-  for (int j = 0; j < n_tiles; ++j) {
-    const int buf = j & 1;
+  for (int j = first; j < n_tiles; ++j) {
+    const int buf = (j - first) & 1;
     if constexpr (sizeof(T) == 4)
       if (bias) {
 #pragma unroll
@@ -371,6 +375,31 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) queries_ker
     __syncthreads();
   }
   cp_wait_all();
+  if constexpr (kSplit) {  // the cluster's parts are added through shared memory, in the order of their keys
+    float *part = reinterpret_cast<float *>(smem4);
+    constexpr int pl = DP + 4;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+        store2(part + (warp * 16 + g + 8 * r) * pl + n * 8 + 2 * t, dq[n][2 * r], dq[n][2 * r + 1]);
+    cluster_barrier();
+    for (int u = rank * threads + tid; u < rows * (DP / 4); u += split * threads) {
+      const int row = u / (DP / 4), c = u % (DP / 4) * 4, i = i0 + row;
+      if (i >= a.nq || c >= a.d) continue;
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < split; ++e) {
+        const float4 w = peer4(reinterpret_cast<const float4 *>(part + row * pl + c), uint32_t(e));
+        y[0] += w.x, y[1] += w.y, y[2] += w.z, y[3] += w.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] *= a.scale;
+      store4(static_cast<T *>(x.dq) + ((int64_t(b) * a.nq + i) * a.heads + h) * a.d + c, y);
+    }
+    cluster_barrier();  // until every part has been read
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = i0 + warp * 16 + g + 8 * r;
@@ -708,9 +737,11 @@ template <typename T, int DP> int launch(const BackArgs &x, cudaStream_t stream)
   if (sizeof(T) == 2)
     if (int rc = queries_tc(x, stream, &taken)) return rc;
   if (!taken) {
-    BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(queries_kernel<T, DP>), 232448));
-    queries_kernel<T, DP>
-        <<<unsigned(ctas), 32 * warps, queries_smem<T, DP>(rows, biased, x.dlow != nullptr), stream>>>(x, int(tiles));
+    const int split = key_split(ctas, (a.nk + kTile<T, DP> - 1) / kTile<T, DP>);
+    auto kernel = split > 1 ? queries_kernel<T, DP, true> : queries_kernel<T, DP, false>;
+    BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(kernel), 232448));
+    BL_CUDA(launch_clusters(kernel, ctas, split, 32 * warps, queries_smem<T, DP>(rows, biased, x.dlow != nullptr), stream, x,
+                            int(tiles), split));
     BL_LAUNCH_CHECK();
   }
   taken = false;

@@ -842,7 +842,7 @@ bool back_maps(CUtensorMap (&m)[6], const BackArgs &x, bool queries_resident) {
 }
 
 bool back_covered(const Args &a) {
-  return a.nk >= 64 && a.nq >= 64 && !(a.bias && !a.bias_vec) && a.batch > 0;
+  return a.nk >= 64 && worth_tiles(a) && !(a.bias && !a.bias_vec) && a.batch > 0;
 }
 
 template <typename K> int back_launch(K kernel, int bytes, const BackTc &p, int64_t ctas, const CUtensorMap (&m)[6], cudaStream_t stream) {

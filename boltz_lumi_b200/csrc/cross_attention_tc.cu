@@ -559,7 +559,8 @@ int launch_tc(const Args &a, const CUtensorMap (&maps)[4], cudaStream_t stream) 
 // Runs the tensor-core kernel and sets *taken where it covers the call.
 int forward_tc(const Args &a, cudaStream_t stream, bool *taken) {
   *taken = false;
-  if (a.nq < 65 || a.nk < 64 || !(a.scale > 0.f) || (a.bias && !a.bias_vec)) return BL_OK;
+  if (a.nk < 64 || !(a.scale > 0.f) || (a.bias && !a.bias_vec)) return BL_OK;
+  if (!worth_tiles(a)) return BL_OK;
   CUtensorMap maps[4];
   const int kv_heads = a.heads / a.group;
   if (!rows_map(&maps[0], a.q, a.d, a.nq, a.heads, a.batch, kBQ) ||

@@ -114,6 +114,12 @@ __device__ __forceinline__ uint32_t mask_word(const Args &a, int b, int w) {
   }
   return word;
 }
+// At most 64 queries leave half or more of a tile's rows idle: worth it over many keys while the heads do not fill
+// the GPU.  32 queries to 4096 keys, forward and gradients in us, against the kernels on warp products: 8 heads 19 / 89
+// against 144 / 201, 64 heads 49 / 182 against 148 / 267, 512 heads 299 / 985 against 133 / 520; equal at 128 keys.
+inline bool worth_tiles(const Args &a) {
+  return a.nq > 64 || (a.nk >= 256 && int64_t(a.heads) * a.batch <= num_sms());
+}
 // Map of a [batch][rows][heads][d] view: box of 64 columns x box_rows rows; false where TMA cannot describe it.
 bool rows_map(CUtensorMap *map, const Rows &r, int d, int rows, int heads, int batch, int box_rows) {
   const int64_t strides[3] = {r.si, r.sh, r.sb};

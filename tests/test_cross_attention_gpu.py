@@ -137,6 +137,20 @@ def test_long_keys(case, dtype):
     test_values_and_gradients(case, dtype)
 
 
+FEW = [
+    (1, 20, 1100, 4, 2, 64, 1, True, "tail"),
+    (2, 33, 700, 2, 2, 48, 2, False, "keep"),
+    (1, 17, 4000, 8, 8, 128, 0, True, "add"),
+    (20, 40, 300, 8, 8, 32, 5, True, "keep"),
+]
+
+
+@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_queries_many_keys(case, dtype):
+    test_values_and_gradients(case, dtype)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [48, 128])
 def test_long_keys_left_out(dtype, d):
