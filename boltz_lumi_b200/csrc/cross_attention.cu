@@ -2,8 +2,10 @@
 //
 // flash_kernel: one CTA = up to 64 query rows of one (sample, head), 16 per
 // warp; key tiles of kBN stream through a two-stage cp.async ring (K, V, the
-// bias block) while the previous tile is computed; running maximum and sum in
-// fp32 registers; the [Nq, Nk] scores never exist in memory.
+// bias block in bf16) while the previous tile is computed; running maximum and sum in
+// fp32 registers; the [Nq, Nk] scores never exist in memory.  Few CTAs become clusters
+// that divide the keys.  640 fp32 windows of 32 x 128, 4 heads of 32: 59 us (floor 19 us: 124 MB);
+// bound by the issue of the split products and their latency at 18 warps per SM.
 #include <array>
 
 #include "cross_attention.cuh"
@@ -278,6 +280,8 @@ template <typename T, int DP> int launch_flash(const Args &a, cudaStream_t strea
 // ring of its own (no CTA barrier in the loop) and keeps its own maximum, sum
 // and output.  The warps' parts are merged in shared memory, the CTAs' parts
 // through distributed shared memory: one launch, no workspace, fixed order.
+// Bound by reading K and V once: 84 MB (5 samples, 16 heads on 4, 16384 keys of 64) in 29 us,
+// 2.9 TB/s; a call of a few us ends before HBM is at its rate.
 // ---------------------------------------------------------------------------
 constexpr int kStepRows = 16;
 

@@ -14,7 +14,14 @@
 //                  summed over the query tiles of every head that shares them;
 //   queries_kernel one CTA = up to 64 query rows of one (sample, head): dq, and
 //                  dbias where no other sample shares the bias;
-//   bias_kernel    one CTA = one block of a shared bias: dbias summed over its samples.
+//   bias_kernel    one CTA = one block of a shared bias: dbias summed over its samples;
+//   window_kernel  all four gradients of small fp32 windows at once.
+// bf16 over 64 queries goes to cross_attention_backward_tc.cu (measured there).  What bounds these
+// kernels is the issue of the warp products: in fp32 each is three (tf32 pairs), and a CTA's
+// 16-row products read and split every operand tile again (10 x 8 x 96 x 6619 x 48, fp32, one bias
+// per five samples: 2.1 ms, 11 TFLOP/s of the formula's products; the plain form's library products
+// take about as long there and at d = 128).  Half the tile (16 rows) at d = 128, for two CTAs per SM, was
+// faster with few queries (961 -> 783 us) and slower else (1715 -> 1960 us).
 #include "cross_attention_backward.cuh"
 
 namespace bl {

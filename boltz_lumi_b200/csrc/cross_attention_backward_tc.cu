@@ -8,13 +8,21 @@
 //                      every head that reads them: S^T = K Q^T and dP^T = V dO^T, P^T and dS^T as
 //                      bf16 in TMEM, dV += P^T dO, dK += dS^T Q (a gated dO in two bf16 terms).
 //
-// Both: warp 0 feeds the tiles by TMA, warp 1 issues the MMAs, warps 4..11 own half a TMEM lane's
-// columns per thread (lane = the resident row).  A tile's scores go to registers at once, so the
-// next tile's products run under this tile's arithmetic.  There is no row maximum to agree on:
-// the forward's statistics give p directly.  A gated do enters dP and dV as two bf16 terms.
-// Against the same loops on mma.sync (measured in cross_attention_backward.cu's comment) they
-// gain because the 16-row warp products there re-read every operand tile from shared memory
-// once per 16 rows.
+//   bias_tc_kernel     the gradient of a bias that several samples share (see there).
+//
+// Both: warp 0 feeds the tiles by TMA; warps 1 to 3 issue the MMAs of the scores, of dP and of the
+// gradients (an MMA of 64 columns costs its issuer 50 to 90 cycles, so one issuer was the limit: 179
+// against 133 us for dQ at 4 x 16 x 777 x 2048 x 128); warps 4..7 and 8..11 take turns over the
+// tiles, a thread per resident row (TMEM lane), in two halves of 32 scores.  S and dP have two
+// buffers, so one set's products run under the other's arithmetic.  There is no row maximum to
+// agree on: the forward's statistics give p directly.  A gated do enters dP and dV as two bf16 terms.
+//
+// Against the same loops on warp products: 4 x 16(4) x 777 x 2048 x 128 without bias, dk/dv 446 ->
+// 138 us, dq 435 -> 133 us (five products, 620 TFLOP/s); 2 x 16 x 384 x 1734 x 48 with a shared bias and a
+// gate, dk/dv 72 -> 48 us, dq 97 -> 35 us, dbias 87 -> 36 us.  What bounds them: at d = 128 the MMAs' operands (an
+// SS product of 64 columns reads 6 KB of shared memory in 48 cycles) beside 2 x 900 cycles of
+// exponentials and conversions per tile and set; at d = 48 that arithmetic and a CTA's start and end,
+// some 8000 of 59000 cycles; CTAs come in whole waves (448 over 148 SMs: four).
 #include "cross_attention_backward.cuh"
 #include "cross_attention_tc.cuh"
 
@@ -204,15 +212,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int bs = j % BS;
 #pragma unroll 1
       for (int half = 0; half < 2 && ok; ++half) {
-      const int k0 = j * kTileTc + 32 * half;
-      uint32_t cut = 0;
-      if (a.mask_kind == kMaskNone) {
-        const int left = a.nk - k0;
-        if (left < 32) cut = left <= 0 ? ~0u : ~0u << left;
-      } else if (use_bits) {
-        cut = bits[2 * j + half];
-      } else {
-        cut = __ballot_sync(0xffffffffu, mask_value(a, b, k0 + lane) != 0.f);
+        const int k0 = j * kTileTc + 32 * half;
+        uint32_t cut = 0;
+        if (a.mask_kind == kMaskNone) {
+          const int left = a.nk - k0;
+          if (left < 32) cut = left <= 0 ? ~0u : ~0u << left;
+        } else if (use_bits) {
+          cut = bits[2 * j + half];
+        } else {
+          cut = __ballot_sync(0xffffffffu, mask_value(a, b, k0 + lane) != 0.f);
       }
       const bool adds = cut && a.mask_kind == kMaskAdd;
       if (adds) {
@@ -536,26 +544,26 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       tc::tc_fence_after();
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-      uint32_t sv[32], dv[32];
-      tc::tmem_ld_32x32b_x32(pair + kSCol + 32 * half, sv);
-      tc::tmem_ld_32x32b_x32(pair + kDpCol + 32 * half, dv);
-      tc::tmem_ld_wait_regs(sv, dv);
-      const float *st = stats + s * 4 * kTileTc + 32 * half;
-      const bool lowest = lowest_flag[4 * s] != 0;
-      // bias(q, key): 64-key block row / 64, row q of 128 bytes, 16-byte chunk (key / 8) ^ (q & 7).
-      const uint8_t *bias = smem + S::kBiasOff + s * S::kB + (row >> 6) * kTileTc * 128 + 32 * half * 128 + (row & 7) * 2;
-      const int chunk = (row & 63) >> 3;
-      uint32_t pt[16], ds[16];
-      uint64_t z[16];
+        uint32_t sv[32], dv[32];
+        tc::tmem_ld_32x32b_x32(pair + kSCol + 32 * half, sv);
+        tc::tmem_ld_32x32b_x32(pair + kDpCol + 32 * half, dv);
+        tc::tmem_ld_wait_regs(sv, dv);
+        const float *st = stats + s * 4 * kTileTc + 32 * half;
+        const bool lowest = lowest_flag[4 * s] != 0;
+        // bias(q, key): 64-key block row / 64, row q of 128 bytes, 16-byte chunk (key / 8) ^ (q & 7).
+        const uint8_t *bias = smem + S::kBiasOff + s * S::kB + (row >> 6) * kTileTc * 128 + 32 * half * 128 + (row & 7) * 2;
+        const int chunk = (row & 63) >> 3;
+        uint32_t pt[16], ds[16];
+        uint64_t z[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if constexpr (kBias) {
-          const uint32_t b0 = *reinterpret_cast<const uint16_t *>(bias + (2 * e) * 128 + ((chunk ^ ((2 * e) & 7)) << 4));
-          const uint32_t b1 = *reinterpret_cast<const uint16_t *>(bias + (2 * e + 1) * 128 + ((chunk ^ ((2 * e + 1) & 7)) << 4));
-          z[e] = add2(fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(b0 << 16, b1 << 16)), mk2);
-        } else {
-          z[e] = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, mk2);
-        }
+        for (int e = 0; e < 16; ++e) {
+          if constexpr (kBias) {
+            const uint32_t b0 = *reinterpret_cast<const uint16_t *>(bias + (2 * e) * 128 + ((chunk ^ ((2 * e) & 7)) << 4));
+            const uint32_t b1 = *reinterpret_cast<const uint16_t *>(bias + (2 * e + 1) * 128 + ((chunk ^ ((2 * e + 1) & 7)) << 4));
+            z[e] = add2(fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, pack2(b0 << 16, b1 << 16)), mk2);
+          } else {
+            z[e] = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, mk2);
+          }
       }
       if (lowest)
 #pragma unroll
@@ -627,7 +635,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 
 // Gradient of a bias that several samples share: one CTA = 128 query rows of one (bias, head) over a
 // range of key tiles; for each tile the samples' Q, dO, K and V stream through a three-stage ring and the
-// threads add up dS in registers.  d <= 64 (two 64-column blocks would leave one stage).
+// threads add up dS in registers.  Bound by those reads from L2 (64 KB per 128 x 64 scores, some 6 TB/s).  d <= 64 (two 64-column blocks would leave one stage).
 template <bool kLow> struct BShape {
   static constexpr int kRes = kRowsTc * 128, kStr = kTileTc * 128, kPer = kLow ? 3 : 2;
   static constexpr int kStage = kPer * kRes + 2 * kStr;  // Q, dO, do - bf16(do), K, V
