@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 
 // Gradient of a bias that several samples share: one CTA = 128 query rows of one (bias, head) over a
 // range of key tiles; for each tile the samples' Q, dO, K and V stream through a three-stage ring and the
-// threads add up dS in registers.  Bound by those reads from L2 (64 KB per 128 x 64 scores, some 6 TB/s).  d <= 64 (two 64-column blocks would leave one stage).
+// threads add up dS in registers.  Bound by those reads from L2 (64 KB per 128 x 64 scores, some 5 TB/s).  d <= 64 (two 64-column blocks would leave one stage).
 template <bool kLow> struct BShape {
   static constexpr int kRes = kRowsTc * 128, kStr = kTileTc * 128, kPer = kLow ? 3 : 2;
   static constexpr int kStage = kPer * kRes + 2 * kStr;  // Q, dO, do - bf16(do), K, V

@@ -14,8 +14,8 @@
 // Both forwards are bound by their HBM writes and both gradients by reading
 // the upstream gradient once.  Encoding of 512 tokens, 128 fp32 channels: 31 us for 134 MB (4.3 TB/s; a plain
 // fill of the same tensor 21 us; the table's load and the launch are the rest).  Its gradient at 424 tokens: 54 us
-// for 92 MB, of which the partial sums' kernel is 8 us; a CTA's private tables leave 12 warps per SM to cover
-// the loads.  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
+// for 92 MB, of which the partial sums' kernel is 8 us; three private tables of 71 KB leave three warps per SM, whose
+// table updates are the limit.  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
 // Table gradient of 2 x 16 x 768 x 1134 fp32: 47 us for 112 MB, 12 us of it clearing and adding up the histograms.  The gradients are deterministic: every partial
 // sum belongs to one thread, and partials are added in a fixed order.
 #include <type_traits>
