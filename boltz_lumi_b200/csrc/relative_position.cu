@@ -13,9 +13,9 @@
 //
 // Both forwards are bound by their HBM writes and both gradients by reading
 // the upstream gradient once.  Encoding of 512 tokens, 128 fp32 channels: 31 us for 134 MB (4.3 TB/s; a plain
-// fill of the same tensor 21 us; the table's load and the launch are the rest).  Its gradient at 424 tokens: 54 us
-// for 92 MB, of which the partial sums' kernel is 8 us; three private tables of 71 KB leave three warps per SM, whose
-// table updates are the limit.  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
+// fill of the same tensor 21 us; the table's load and the launch are the rest).  Its gradient at 424 tokens: 40 us
+// for 92 MB, of which the partial sums' kernel is 4 us; six private tables of 36 KB leave six warps per SM, whose
+// instructions are the limit.  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
 // Table gradient of 2 x 16 x 768 x 1134 fp32: 47 us for 112 MB, 12 us of it clearing and adding up the histograms.  The gradients are deterministic: every partial
 // sum belongs to one thread, and partials are added in a fixed order.
 #include <type_traits>
@@ -154,43 +154,43 @@ __global__ void __launch_bounds__(1024) encoding_kernel(const float *w, const En
   }
 }
 
-// Gradient of W.  A warp covers 128 channels (four per lane) and owns a private
-// [rows][128] table in shared memory, each element of which one lane alone
+// Gradient of W.  A warp covers 64 channels (two per lane) and owns a private
+// [rows][64] table in shared memory, each element of which one lane alone
 // updates.  It walks diagonals: from pair (i0, j) it visits (i0 + s, (j + s) mod n)
 // for up to kSteps rows, every load a whole pair row, two walks' loads in flight at
 // once.  Along a diagonal of one chain the offsets, so the picks, do not change: the
 // sum of the pairs stays in registers and goes to the table rows of its picks when one
 // of them changes.
-constexpr int kGroups = 3;  // private tables per CTA (71 KB each at r = 32, s = 2)
-template <typename In> constexpr int kSteps = sizeof(In) == 4 ? 16 : 32;
+// (128 channels per warp leave three warps per SM: 53 us at 424 tokens in fp32, 57 in bf16, against 40 and 39.)
+constexpr int kGradCh = 64, kGroups = 6;  // private tables per CTA (36 KB each at r = 32, s = 2)
+constexpr int kSteps = 16;
 
-__device__ __forceinline__ float4 as_float4(float4 v) { return v; }
-__device__ __forceinline__ float4 as_float4(uint2 v) {
-  return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
-}
+__device__ __forceinline__ float2 as_float2(float2 v) { return v; }
+__device__ __forceinline__ float2 as_float2(uint32_t v) { return make_float2(bf16_lo(v), bf16_hi(v)); }
+__device__ __forceinline__ float2 sum2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
 
 template <typename In>
 __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *grad, const EncArgs a, float *partial) {
-  constexpr int kS = kSteps<In>;
-  using Raw = typename std::conditional<sizeof(In) == 4, float4, uint2>::type;
+  constexpr int kS = kSteps;
+  using Raw = typename std::conditional<sizeof(In) == 4, float2, uint32_t>::type;
   extern __shared__ float4 smem4[];
   float *tables = reinterpret_cast<float *>(smem4);
-  const int groups = blockDim.x / 32, size = a.rows * 128;
+  const int groups = blockDim.x / 32, size = a.rows * kGradCh;
   for (int i = threadIdx.x; i < groups * size / 4; i += blockDim.x) smem4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   __syncthreads();
-  const int lane = threadIdx.x & 31, group = threadIdx.x / 32, ch = 4 * lane, c0 = blockIdx.y * 128;
+  const int lane = threadIdx.x & 31, group = threadIdx.x / 32, ch = 2 * lane, c0 = blockIdx.y * kGradCh;
   const bool live = c0 + ch < a.channels;  // channels is a multiple of 4
-  float4 *mine = reinterpret_cast<float4 *>(tables + group * size + ch);
+  float2 *mine = reinterpret_cast<float2 *>(tables + group * size + ch);
   const int n = a.n, blocks = (n + kS - 1) / kS;
   const uint32_t units = uint32_t(a.batch * blocks * n);
   const int64_t step = (int64_t(n) + 1) * a.channels, wrap = int64_t(n) * a.channels;
-  float4 run = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 run = make_float2(0.f, 0.f);
   uint32_t held = 0xffffffffu;
-  auto put = [&](uint32_t row) { mine[row * 32] = add4(mine[row * 32], run); };
+  auto put = [&](uint32_t row) { mine[row * 32] = sum2(mine[row * 32], run); };
   auto flush = [&]() {
     put(held & 1023u), put((held >> 10) & 1023u), put((held >> 20) & 1023u);
     if (held >> 30) put(4 * a.r + 4);
-    run = make_float4(0.f, 0.f, 0.f, 0.f);
+    run = make_float2(0.f, 0.f);
   };
   struct Walk {
     Raw x[kS];
@@ -205,12 +205,17 @@ __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *g
     const In *p = grad + ((b0 + i0) * n + j) * a.channels + c0 + ch;
     const int turn = n - j;  // first step past the row's end (s < count <= n: at most one turn)
     const int last = live ? w.count : 0;
+    if (last == kS && turn >= kS) {
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      if (s == turn) p -= wrap;
-      w.x[s] = {};
-      if (s < last) w.x[s] = __ldcs(reinterpret_cast<const Raw *>(p));
-      p += step;
+      for (int s = 0; s < kS; ++s, p += step) w.x[s] = __ldcs(reinterpret_cast<const Raw *>(p));
+    } else {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        if (s == turn) p -= wrap;
+        w.x[s] = {};
+        if (s < last) w.x[s] = __ldcs(reinterpret_cast<const Raw *>(p));
+        p += step;
+      }
     }
     const int col = j + lane >= n ? j + lane - n : j + lane;
     if (lane < w.count) w.f = pair_features(a, b0 + i0 + lane, b0 + col);
@@ -224,10 +229,10 @@ __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *g
         if (held != 0xffffffffu) flush();
         held = first;
       }
-      float4 part = make_float4(0.f, 0.f, 0.f, 0.f);
+      float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int s = 0; s < kS; ++s) part = add4(part, as_float4(w.x[s]));
-      run = add4(run, part);
+      for (int s = 0; s < kS; ++s) part = sum2(part, as_float2(w.x[s]));
+      run = sum2(run, part);
     } else {
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *g
             if (held != 0xffffffffu) flush();
             held = v;
           }
-          run = add4(run, as_float4(w.x[s]));
+          run = sum2(run, as_float2(w.x[s]));
         }
       }
     }
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *g
   }
   if (held != 0xffffffffu) flush();
   __syncthreads();
-  // partial[cta][channel chunk][row][128]
+  // partial[cta][channel chunk][row][kGradCh]
   float4 *dst = reinterpret_cast<float4 *>(partial + (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * size);
   for (int i = threadIdx.x; i < size / 4; i += blockDim.x) {
     float4 v = smem4[i];
@@ -263,12 +268,12 @@ __global__ void __launch_bounds__(kGroups * 32) encoding_grad_kernel(const In *g
   }
 }
 
-// dw[c][row] = sum over CTAs of partial[cta][c / 128][row][c % 128]; 8 threads per output, joined in a fixed order.
+// dw[c][row] = sum over CTAs of partial[cta][c / kGradCh][row][c % kGradCh]; 8 threads per output, joined in a fixed order.
 __global__ void __launch_bounds__(256) encoding_grad_sum_kernel(const float *partial, int ctas, int chunks, int rows,
                                                                 int channels, float *dw) {
   __shared__ float part[8][33];
   const int lane = threadIdx.x & 31, way = threadIdx.x >> 5;
-  const int64_t size = int64_t(chunks) * rows * 128;
+  const int64_t size = int64_t(chunks) * rows * kGradCh;
   const int64_t at = int64_t(blockIdx.x) * 32 + lane;
   float v = 0.f;
   if (at < size)
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(256) encoding_grad_sum_kernel(const float *par
   __syncthreads();
   if (way == 0 && at < size) {
     for (int k = 1; k < 8; ++k) v += part[k][lane];
-    const int c = int(at / (int64_t(rows) * 128)) * 128 + int(at % 128), row = int(at / 128 % rows);
+    const int c = int(at / (int64_t(rows) * kGradCh)) * kGradCh + int(at % kGradCh), row = int(at / kGradCh % rows);
     if (c < channels) dw[int64_t(c) * rows + row] = v;
   }
 }
@@ -293,11 +298,11 @@ int encoding_check(const char *name, const EncArgs &a, int64_t n, int64_t channe
 }
 
 int encoding_grad_groups(int rows) {  // private tables that fit in 227 KB
-  const int fit = kMaxSmem / (rows * 128 * 4);
+  const int fit = kMaxSmem / (rows * kGradCh * 4);
   return fit < kGroups ? fit : kGroups;
 }
 int64_t encoding_grad_ctas(int64_t batch, int64_t n, int rows, int chunks) {
-  const int64_t units = batch * ((n + 15) / 16) * n, groups = encoding_grad_groups(rows);
+  const int64_t units = batch * ((n + kSteps - 1) / kSteps) * n, groups = encoding_grad_groups(rows);
   const int64_t want = (units + groups - 1) / groups, cap = (num_sms() + chunks - 1) / chunks;
   return want < 1 ? 1 : want < cap ? want : cap;
 }
@@ -676,8 +681,8 @@ extern "C" int bl_relative_position_encoding(const float *weight, const int64_t 
 extern "C" int64_t bl_relative_position_encoding_workspace(int64_t batch, int64_t n, int64_t channels, int64_t r_max,
                                                            int64_t s_max) {
   if (batch <= 0 || n <= 0 || channels <= 0 || r_max < 0 || s_max < 0 || r_max > 96 || s_max > 16) return 0;
-  const int rows = int(4 * r_max + 2 * s_max + 7), chunks = int((channels + 127) / 128);
-  return encoding_grad_ctas(batch, n, rows, chunks) * chunks * rows * 128 * 4;
+  const int rows = int(4 * r_max + 2 * s_max + 7), chunks = int((channels + kGradCh - 1) / kGradCh);
+  return encoding_grad_ctas(batch, n, rows, chunks) * chunks * rows * kGradCh * 4;
 }
 
 extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtype, const int64_t *residue,
@@ -700,9 +705,9 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
   const int64_t need = bl_relative_position_encoding_workspace(batch, n, channels, r_max, s_max);
   BL_REQUIRE(workspace && workspace_bytes >= need && aligned_to(workspace, 16),
              "bl_relative_position_encoding_backward: needs a workspace of %lld bytes", (long long)need);
-  const int chunks = int((channels + 127) / 128), groups = encoding_grad_groups(a.rows);
+  const int chunks = int((channels + kGradCh - 1) / kGradCh), groups = encoding_grad_groups(a.rows);
   const int64_t ctas = encoding_grad_ctas(batch, n, a.rows, chunks);
-  const int smem = groups * a.rows * 128 * 4;
+  const int smem = groups * a.rows * kGradCh * 4;
   float *part = static_cast<float *>(workspace);
   dim3 grid{unsigned(ctas), unsigned(chunks)};
   if (dtype == BL_F32) {
@@ -714,7 +719,7 @@ extern "C" int bl_relative_position_encoding_backward(const void *grad, int dtyp
         <<<grid, groups * 32, smem, st>>>(static_cast<const __nv_bfloat16 *>(grad), a, part);
   }
   BL_LAUNCH_CHECK();
-  const int64_t size = int64_t(chunks) * a.rows * 128;
+  const int64_t size = int64_t(chunks) * a.rows * kGradCh;
   encoding_grad_sum_kernel<<<unsigned((size + 31) / 32), 256, 0, st>>>(part, int(ctas), chunks, a.rows, a.channels,
                                                                        dweight);
   BL_LAUNCH_CHECK();
