@@ -169,6 +169,14 @@ def test_long_keys_left_out(dtype, d):
     check(actual, *reference(**x))
 
 
+@pytest.mark.parametrize("d", [48, 128])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("share", [0, 1, 2])
+def test_many_tiles(d, gate, share):
+    """Every variant of the tensor-core kernels over rings that turn several times, in both directions."""
+    test_values_and_gradients((2, 650, 710, 4, 2, d, share, gate, "keep"), torch.bfloat16)
+
+
 @pytest.mark.parametrize("d", range(8, 129, 8))
 def test_head_dims(d):
     test_values_and_gradients((2, 70, 80, 2, 1, d, 2, d % 16 == 0, "keep"), torch.bfloat16)
