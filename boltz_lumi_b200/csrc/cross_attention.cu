@@ -280,8 +280,8 @@ template <typename T, int DP> int launch_flash(const Args &a, cudaStream_t strea
 // ring of its own (no CTA barrier in the loop) and keeps its own maximum, sum
 // and output.  The warps' parts are merged in shared memory, the CTAs' parts
 // through distributed shared memory: one launch, no workspace, fixed order.
-// Bound by reading K and V once: 84 MB (5 samples, 16 heads on 4, 16384 keys of 64) in 29 us,
-// 2.9 TB/s; a call of a few us ends before HBM is at its rate.
+// Bound by reading K and V once: 84 MB (5 samples, 16 heads on 4, 16384 keys of 64) in 25 us,
+// 3.3 TB/s; clusters of 6 cover 120 of the 148 SMs, and a call of a few us ends before HBM is at its rate.
 // ---------------------------------------------------------------------------
 constexpr int kStepRows = 16;
 
@@ -296,7 +296,10 @@ template <typename T, int DP> struct Step {
   static constexpr int q_bytes = kStepRows * ld * int(sizeof(T));
   static constexpr int ring_bytes = warps * stages * stage_bytes;
   static constexpr int part_bytes = (warps * kStepRows * (DP + 2) + 2 * kStepRows) * 4;
-  static constexpr int bytes = q_bytes + (ring_bytes > part_bytes ? ring_bytes : part_bytes);
+  static constexpr int bits_off = q_bytes + (ring_bytes > part_bytes ? ring_bytes : part_bytes);
+  // Keep mask of the CTA's keys as bits, where it fits.
+  static constexpr int mask_words = (232448 - bits_off) / 4 < 2048 ? (232448 - bits_off) / 4 : 2048;
+  static constexpr int bytes = bits_off + mask_words * 4;
 };
 
 template <typename T, int DP>
@@ -322,17 +325,26 @@ __global__ void __launch_bounds__(32 * Step<T, DP>::warps) step_kernel(const Arg
   }
   cp_commit();
   const int64_t chunks = (a.nk + KC - 1) / KC;
-  const int c_end = int((rank + 1) * chunks / split);
-  int next = int(rank * chunks / split) + warp;  // chunk to issue
+  const int c_begin = int(rank * chunks / split), c_end = int((rank + 1) * chunks / split);
+  // The mask decides which rows are loaded, so it has to be there ahead of them: read chunk by chunk it cost
+  // 6 of 29 us at 5 samples of 16384 keys.
+  uint32_t *bits = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(smem4) + S::bits_off);
+  const int w0 = int(int64_t(c_begin) * KC / 32), words = int((int64_t(c_end) * KC + 31) / 32) - w0;
+  const bool use_bits = a.mask_kind == kMaskKeep && words <= S::mask_words;
+  int next = c_begin + warp;  // chunk to issue
   float mk_next = lane < KC && next < c_end ? mask_value(a, b, next * KC + lane) : -INFINITY;
   int put = 0;
   // Keys that are left out are not loaded: their rows are zero whatever they hold.
-  auto issue = [&]() {
+  auto issue = [&](bool first) {
     if (next < c_end) {
       char *st = mine + put * S::stage_bytes;
       T *kt = reinterpret_cast<T *>(st), *vt = kt + S::kv, *bt = vt + S::kv;
       float *mk = reinterpret_cast<float *>(bt + S::bias);
       const int j0 = next * KC;
+      if (use_bits && !first) {
+        const int j = next * KC;
+        mk_next = bits[(j >> 5) - w0] >> ((j & 31) + (lane & (KC - 1))) & 1 ? -INFINITY : 0.f;
+      }
       if (lane < KC) mk[lane] = mk_next;
       // Lane: chunk c of rows r0, r0 + kStep, ...
       constexpr int kStep = 32 / kChunks > 0 ? 32 / kChunks : 1;
@@ -361,22 +373,24 @@ __global__ void __launch_bounds__(32 * Step<T, DP>::warps) step_kernel(const Arg
         }
       }
       next += kStepWarps;
-      mk_next = lane < KC && next < c_end ? mask_value(a, b, next * KC + lane) : -INFINITY;
+      if (!use_bits || first) mk_next = lane < KC && next < c_end ? mask_value(a, b, next * KC + lane) : -INFINITY;
     }
     cp_commit();
     put = put + 1 == kStepStages ? 0 : put + 1;
   };
 #pragma unroll
-  for (int e = 0; e < kStepStages - 1; ++e) issue();
+  for (int e = 0; e < kStepStages - 1; ++e) issue(true);
+  if (use_bits)
+    for (int w = tid; w < words; w += 32 * kStepWarps) bits[w] = mask_word(a, b, w0 + w);
   cp_wait<kStepStages - 1>();
-  __syncthreads();  // Q
+  __syncthreads();  // Q and the mask
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[ND][4];
 #pragma unroll
   for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   int take = 0;
-  for (int c = int(rank * chunks / split) + warp; c < c_end; c += kStepWarps) {
-    issue();
+  for (int c = c_begin + warp; c < c_end; c += kStepWarps) {
+    issue(false);
     cp_wait<kStepStages - 1>();
     __syncwarp();
     const char *st = mine + take * S::stage_bytes;

@@ -145,6 +145,29 @@ __device__ __forceinline__ float mask_value(const Args &a, int b, int j) {
   return a.inf * (static_cast<const float *>(a.mask)[b * a.mask_sb + j] - 1.f);
 }
 
+// Bits of keys [32 w, 32 w + 32): left out by a keep mask, changed by an additive one, or past nk.
+__device__ __forceinline__ uint32_t mask_word(const Args &a, int b, int w) {
+  uint32_t word = 0;
+  const int j0 = 32 * w;
+  if (a.mask_kind == kMaskKeep) {
+    const uint8_t *m = static_cast<const uint8_t *>(a.mask) + b * a.mask_sb + j0;
+    if (j0 + 32 <= a.nk && (reinterpret_cast<uintptr_t>(m) & 15) == 0) {
+      const uint4 v[2] = {reinterpret_cast<const uint4 *>(m)[0], reinterpret_cast<const uint4 *>(m)[1]};
+      const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // 0xff where a byte is zero; its low bits gathered to four
+        word |= ((__vcmpeq4(u[e], 0u) & 0x01010101u) * 0x10204080u >> 28) << (4 * e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) word |= uint32_t(j0 + e >= a.nk || m[e] == 0) << e;
+    }
+  } else {
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) word |= uint32_t(mask_value(a, b, j0 + e) != 0.f) << e;
+  }
+  return word;
+}
+
 // Two neighbouring elements of a shared row.
 __device__ __forceinline__ float2 load2(const float *p) { return *reinterpret_cast<const float2 *>(p); }
 __device__ __forceinline__ float2 load2(const __nv_bfloat16 *p) {

@@ -92,28 +92,6 @@ __device__ __forceinline__ void mma_cols_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 }
 
 __device__ __forceinline__ int n_words(int nk) { return (nk + 31) / 32; }
-// Bits of keys [32 w, 32 w + 32): left out by a keep mask, changed by an additive one, or past nk.
-__device__ __forceinline__ uint32_t mask_word(const Args &a, int b, int w) {
-  uint32_t word = 0;
-  const int j0 = 32 * w;
-  if (a.mask_kind == kMaskKeep) {
-    const uint8_t *m = static_cast<const uint8_t *>(a.mask) + b * a.mask_sb + j0;
-    if (j0 + 32 <= a.nk && (reinterpret_cast<uintptr_t>(m) & 15) == 0) {
-      const uint4 v[2] = {reinterpret_cast<const uint4 *>(m)[0], reinterpret_cast<const uint4 *>(m)[1]};
-      const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)  // 0xff where a byte is zero; its low bits gathered to four
-        word |= ((__vcmpeq4(u[e], 0u) & 0x01010101u) * 0x10204080u >> 28) << (4 * e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) word |= uint32_t(j0 + e >= a.nk || m[e] == 0) << e;
-    }
-  } else {
-#pragma unroll 8
-    for (int e = 0; e < 32; ++e) word |= uint32_t(mask_value(a, b, j0 + e) != 0.f) << e;
-  }
-  return word;
-}
 // At most 64 queries leave half or more of a tile's rows idle: worth it over many keys while the heads do not fill
 // the GPU.  32 queries to 4096 keys, forward and gradients in us, against the kernels on warp products: 8 heads 19 / 89
 // against 144 / 201, 64 heads 49 / 182 against 148 / 267, 512 heads 299 / 985 against 133 / 520; equal at 128 keys.
