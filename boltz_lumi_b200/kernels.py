@@ -395,22 +395,23 @@ def _workspace(nbytes, device):
     return torch.empty(max(int(nbytes), 16), device=device, dtype=torch.uint8)
 
 
-def _indices(device, shape, **tensors):
-    """Integer index tensors as contiguous int64 of ``shape`` on ``device`` (None stays None)."""
-    out = []
-    for name, t in tensors.items():
-        if t is not None:
-            if t.device != device:
-                raise RuntimeError(f"{name} must be on {device}, got {t.device}")
-            if t.shape != shape:
-                raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-            if t.dtype != torch.int64:
-                if t.dtype not in (torch.int32, torch.int16, torch.uint8):
-                    raise RuntimeError(f"{name} must hold integers, got {t.dtype}")
-                t = t.to(torch.int64)
-            t = t.contiguous()
-        out.append(t)
-    return out
+def _index(name, t, device, shape):
+    """An integer index tensor as contiguous int64 of ``shape`` on ``device`` (None stays None)."""
+    if t is None or t.dtype is torch.int64 and t.shape == shape and t.device == device and t.is_contiguous():
+        return t
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+    if t.shape != shape:
+        raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+        raise RuntimeError(f"{name} must hold integers, got {t.dtype}")
+    return t.to(torch.int64).contiguous()
+
+
+def _token_features(device, shape, residue_index, asym_id, entity_id, token_index, sym_id):
+    return (_index("residue_index", residue_index, device, shape), _index("asym_id", asym_id, device, shape),
+            _index("entity_id", entity_id, device, shape), _index("token_index", token_index, device, shape),
+            _index("sym_id", sym_id, device, shape))
 
 
 def _float_dtype(dtype, what):
@@ -448,8 +449,7 @@ def relative_position_encoding(weight, residue_index, asym_id, entity_id, token_
         raise RuntimeError(f"weight must be fp32 [C, {relative_position_columns(r_max, s_max)}] for r_max {r_max}, "
                            f"s_max {s_max}, got {weight.dtype} {list(weight.shape)}")
     c = weight.shape[0]
-    features = _indices(weight.device, (b, n), residue_index=residue_index, asym_id=asym_id, entity_id=entity_id,
-                        token_index=token_index, sym_id=sym_id)
+    features = _token_features(weight.device, (b, n), residue_index, asym_id, entity_id, token_index, sym_id)
     if residual is not None:
         if residual.dtype != torch.float32 or not residual.is_contiguous() or tuple(residual.shape) != (b, n, n, c):
             raise RuntimeError(f"residual must be a contiguous fp32 tensor [{b}, {n}, {n}, {c}]")
@@ -475,8 +475,7 @@ def relative_position_encoding_backward(grad, residue_index, asym_id, entity_id,
     _float_dtype(grad.dtype, "grad")
     b, n, _, c = grad.shape
     device = grad.device
-    features = _indices(device, (b, n), residue_index=residue_index, asym_id=asym_id, entity_id=entity_id,
-                        token_index=token_index, sym_id=sym_id)
+    features = _token_features(device, (b, n), residue_index, asym_id, entity_id, token_index, sym_id)
     grad = grad.contiguous()
     if grad.data_ptr() % 16:
         grad = grad.clone()
@@ -523,15 +522,15 @@ def _bias_positions(device, q_pos, k_pos, lut, q_group, k_group):
         raise RuntimeError("give both q_group and k_group or neither")
     if lut.dim() != 1 or lut.dtype != torch.int32 or lut.numel() % 2 == 0 or lut.device != device:
         raise RuntimeError("lut must be an int32 vector of odd length on the device of the other tensors")
-    qp, qg = _indices(device, q_pos.shape, q_pos=q_pos, q_group=q_group)
-    kp, kg = _indices(device, k_pos.shape, k_pos=k_pos, k_group=k_group)
-    return qp, kp, lut.contiguous(), qg, kg
+    return (_index("q_pos", q_pos, device, q_pos.shape), _index("k_pos", k_pos, device, k_pos.shape), lut.contiguous(),
+            _index("q_group", q_group, device, q_pos.shape), _index("k_group", k_group, device, k_pos.shape))
 
 
 def padded_planes(b, h, nq, nk, device, dtype):
     """An uninitialised [b, h, nq, nk] whose rows start on 16-byte boundaries (the layout the attention kernels
-    read fastest): a view of rows padded to a multiple of 8 elements."""
-    return torch.empty(b, h, nq, (nk + 7) // 8 * 8, device=device, dtype=dtype)[..., :nk]
+    read fastest): rows padded to a multiple of 8 elements."""
+    ld = (nk + 7) // 8 * 8
+    return torch.empty_strided((b, h, nq, nk), (h * nq * ld, nq * ld, ld, 1), device=device, dtype=dtype)
 
 
 def relative_position_bias(table, q_pos, k_pos, lut, q_group=None, k_group=None, out_dtype=None):
