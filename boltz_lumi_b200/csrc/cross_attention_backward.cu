@@ -524,7 +524,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) bias_kernel
 // has query rows 16 (w & 1) and keys 32 (w / 2); P and dS go through shared memory to the keys'
 // products (16 keys per warp), dq is summed over the four key blocks.  The CTA walks the samples
 // that share a bias, dbias stays in its registers.  96 biases x 4 samples of 32 x 128, 4 heads of 32:
-// 76 us (150 with the kernels above); bound by the split products' issue and latency, not by bytes
+// 67 us (150 with the kernels above; 76 with the bias read after the score products); bound by the split products' issue and latency, not by bytes
 // (floor 17 us).
 constexpr int kWinThreads = 256, kWinRows = 32, kWinKeys = 128, kWinLd = kWinKeys + 4;
 
@@ -592,6 +592,15 @@ template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kerne
     load_rows<float, DP, kWinKeys>(ks, k, a.k.si, 0, a.nk, a.d, tid, kWinThreads);
     load_rows<float, DP, kWinKeys>(vs, v, a.v.si, 0, a.nk, a.d, tid, kWinThreads);
     cp_commit();
+    float2 bv[NT][2];  // the bias, in flight under the tiles' copies
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = r0 + g + 8 * r;
+      const float *br = bias + int64_t(i) * a.bias_si + c0 + 2 * t;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        bv[n][r] = bias ? bias_pair(a, br + n * 8, i < a.nq ? a.nk - c0 - n * 8 - 2 * t : 0) : make_float2(0.f, 0.f);
+    }
     bool gone = false;
     if (tid < kWinKeys) {
       const float mk = mask_value(a, b, tid);
@@ -624,14 +633,12 @@ template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kerne
       for (int r = 0; r < 2; ++r) {
         const int i = r0 + g + 8 * r;
         const float m = st[i], nl = st[kWinRows + i], delta = st[2 * kWinRows + i];
-        const float *br = bias ? bias + int64_t(i) * a.bias_si + c0 + 2 * t : nullptr;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int j = c0 + n * 8 + 2 * t;
-          const float2 bv = br ? bias_pair(a, br + n * 8, i < a.nq ? a.nk - j : 0) : make_float2(0.f, 0.f);
           const float2 mk = load2(mks + j);
-          grad_score(s[n][2 * r], dp[n][2 * r], a.scale, bv.x, mk.x, m, nl, delta);
-          grad_score(s[n][2 * r + 1], dp[n][2 * r + 1], a.scale, bv.y, mk.y, m, nl, delta);
+          grad_score(s[n][2 * r], dp[n][2 * r], a.scale, bv[n][r].x, mk.x, m, nl, delta);
+          grad_score(s[n][2 * r + 1], dp[n][2 * r + 1], a.scale, bv[n][r].y, mk.y, m, nl, delta);
         }
       }
 #pragma unroll
@@ -699,8 +706,8 @@ template <int DP> __global__ void __launch_bounds__(kWinThreads, 2) window_kerne
           store_bias(dbias + (r0 + g + 8 * r) * x.dbias_ld, c0 + n * 8 + 2 * t, a.nk, sum[n][2 * r], sum[n][2 * r + 1]);
 }
 
-// *taken where the windows' kernel has run.  At 32 x 128 x 4 heads it takes 13 us against 23 of the kernels above for
-// 4 biases of one sample, 35 against 41 for 16 biases of 4, but a CTA that walks many samples alone is slower (107
+// *taken where the windows' kernel has run.  At 32 x 128 x 4 heads it takes 12 us against 23 of the kernels above for
+// 4 biases of one sample, 30 against 41 for 16 biases of 4, but a CTA that walks many samples alone is slower (107
 // against 60 us for 1 bias of 16).  Below 17 queries or 33 keys half of its warps idle (43 against 39 us at 16 x 33).
 template <int DP> int launch_window(const BackArgs &x, cudaStream_t stream, bool *taken) {
   const Args &a = x.a;
