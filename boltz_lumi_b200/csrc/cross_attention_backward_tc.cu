@@ -200,8 +200,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int64_t at = (int64_t(b) * a.heads + h) * a.nq + i;
       m = row_max(a.lse[at]), nl = -kLog2e * a.lse[a.lse_plane() + at], delta = p.x.delta[at];
     }
-    // A reference of the type's lowest values overflows in base 2: subtract it first there.
-    const bool lowest = __any_sync(0xffffffffu, m < -1e37f);
+    const bool far = __any_sync(0xffffffffu, far_row(m));
     const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta), scale2 = dup2(a.scale);
     const uint64_t log2e2 = dup2(kLog2e);
     Bf *dbias = kBias && p.x.dbias && a.share == 1 && i < a.nq
@@ -261,7 +260,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = add2(y[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
       uint32_t ds[16];
-      if (lowest)
+      if (far)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           y[e] = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
@@ -389,7 +388,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   uint64_t *d_full = pv_done + 2;        // every product is done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_full + 1);
   float *stats = reinterpret_cast<float *>(smem + S::kStatOff);
-  int *lowest_flag = reinterpret_cast<int *>(stats + ST * 4 * kTileTc);  // [ST], 16 bytes apart
+  int *far_flag = reinterpret_cast<int *>(stats + ST * 4 * kTileTc);  // [ST], 16 bytes apart
   const Args &a = p.x.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv_heads = a.heads / a.group;
   int tile, hk, b;
@@ -477,17 +476,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int s = u % ST, set = u & 1;
       if (u >= ST && !(ok = warp_wait(stat_empty + s, ((u / ST) & 1) ^ 1u, p.status, 0x417))) break;
       float *st = stats + s * 4 * kTileTc;
-      bool low = false;
+      bool any_far = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = lane + 32 * e;
         const float top = row_max(m[e]), off = -kLog2e * nl[e];
         st[r] = top, st[kTileTc + r] = off, st[3 * kTileTc + r] = -dl[e];
         st[2 * kTileTc + r] = top == INFINITY ? -INFINITY : fmaf(-top, kLog2e, off);
-        low |= top < -1e37f;
+        any_far |= far_row(top);
       }
-      const bool lowest = __any_sync(0xffffffffu, low);
-      if (lane == 0) lowest_flag[4 * s] = lowest;
+      any_far = __any_sync(0xffffffffu, any_far);
+      if (lane == 0) far_flag[4 * s] = any_far;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(stat_full + s);
       if (u + 1 < n) fetch(u + 1);
@@ -549,7 +548,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         tc::tmem_ld_32x32b_x32(pair + kDpCol + 32 * half, dv);
         tc::tmem_ld_wait_regs(sv, dv);
         const float *st = stats + s * 4 * kTileTc + 32 * half;
-        const bool lowest = lowest_flag[4 * s] != 0;
+        const bool far = far_flag[4 * s] != 0;
         // bias(q, key): 64-key block row / 64, row q of 128 bytes, 16-byte chunk (key / 8) ^ (q & 7).
         const uint8_t *bias = smem + S::kBiasOff + s * S::kB + (row >> 6) * kTileTc * 128 + 32 * half * 128 + (row & 7) * 2;
         const int chunk = (row & 63) >> 3;
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             z[e] = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, mk2);
           }
       }
-      if (lowest)
+      if (far)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
@@ -756,7 +755,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         mk[lane] = mv == -INFINITY ? 0.f : mv;
         __syncwarp();
       }
-      const bool lowest = __any_sync(0xffffffffu, m < -1e37f);
+      const bool far = __any_sync(0xffffffffu, far_row(m));
       const uint64_t c2 = dup2(m == INFINITY ? -INFINITY : fmaf(-m, kLog2e, nl)), delta2 = dup2(-delta);
       const float m_now = m, nl_now = nl;
       if (u + 1 < n) fetch(u + 1);
@@ -784,7 +783,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (adds)
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[e] = add2(z[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
-      if (lowest)
+      if (far)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - m_now, kLog2e, nl_now)), __float_as_uint(fmaf(hi_f(z[e]) - m_now, kLog2e, nl_now)));

@@ -373,8 +373,7 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       // P of tile j - 2 was in this buffer.  Its P.V has read it: it was issued before S of
       // this tile, whose commit (s_full) covers every earlier product of that thread.
       const uint32_t p_col = lanes + S::kPCol + buf * 32;
-      if (__any_sync(0xffffffffu, m < -1e37f && m != -INFINITY)) {
-        // A row of the type's lowest values: subtract before the change of base, which would overflow.
+      if (__any_sync(0xffffffffu, far_row(m))) {
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {

@@ -91,6 +91,13 @@ __device__ __forceinline__ void mma_cols_ts(uint32_t d_tmem, uint32_t a_tmem, ui
   for (int e = 0; e < kSteps; ++e) tc::umma_f16_ts(d_tmem, a_tmem + e * 8, with_low(b + e * 128), idesc, add || e != 0);
 }
 
+// A row whose reference m is far from zero: m is subtracted from its scores before the change of base.  Else -m log2(e) is
+// rounded once into an offset of the exponents (and once more with the log of the sum in the gradients), which costs
+// at most |m| 2^-23 of a probability: 2^-13 here, a 32nd of what rounding it to bf16 does.  Without the limit a sample whose
+// keys are all masked by -1e6 came out 2.3 times further off than its bounds, by -1e9 with gradients of 1e7, by -1e10 as NaN.
+constexpr float kFar = 1024.f;
+__device__ __forceinline__ bool far_row(float m) { return fabsf(m) > kFar && fabsf(m) != INFINITY; }
+
 __device__ __forceinline__ int n_words(int nk) { return (nk + 31) / 32; }
 // At most 64 queries leave half or more of a tile's rows idle: worth it over many keys while the heads do not fill
 // the GPU.  32 queries to 4096 keys, forward and gradients in us, against the kernels on warp products: 8 heads 19 / 89
