@@ -136,7 +136,10 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) keys_kernel
     if (tid < BQ) {
       const int64_t at = (int64_t(b) * a.heads + h) * a.nq;
       const bool ok = i0 + tid < a.nq;
-      cp4(ls + buf * BQ + tid, a.lse + at + (ok ? i0 + tid : 0), ok);
+      if (ok)
+        cp4(ls + buf * BQ + tid, a.lse + at + i0 + tid, true);
+      else  // a row past the last: p = 0 whatever the mask adds (0 for its reference made exp(mask term) of it)
+        ls[buf * BQ + tid] = -INFINITY;
       cp4(lg + buf * BQ + tid, a.lse + a.lse_plane() + at + (ok ? i0 + tid : 0), ok);
       cp4(del + buf * BQ + tid, x.delta + at + (ok ? i0 + tid : 0), ok);
     }

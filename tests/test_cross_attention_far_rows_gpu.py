@@ -105,3 +105,27 @@ def test_bias_rows(shape, shift, dtype):
     terms = [x["bias"].float().repeat_interleave(share, 0)]
     actual = compare(x, *rounded_reference(x, terms), share)
     assert math.isfinite(float(actual["lse"].sum()))
+
+
+ABOVE_ONE = [
+    # b, nq, nk, h, hk, d, share, gate: query rows that do not fill the gradient kernels' tiles
+    (2, 37, 70, 2, 1, 32, 1, True),
+    (2, 37, 70, 2, 2, 128, 0, False),
+    (4, 20, 96, 2, 2, 32, 2, True),  # fp32: the windows' kernel
+    (1, 130, 200, 2, 1, 48, 1, True),
+    (2, 3, 90, 4, 2, 64, 1, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", ABOVE_ONE)
+def test_additive_masks_above_one(shape, dtype):
+    """A mask of 2 adds inf to a key's scores: query rows past the last one must not see it."""
+    b, nk, share = shape[0], shape[2], shape[6]
+    x = exact_inputs(shape, dtype)
+    x["mask"], x["inf"] = torch.ones(b, nk), 1e3
+    x["mask"][:, 5], x["mask"][:, nk - 1], x["mask"][:, 7] = 2.0, 2.0, 0.0
+    terms = [torch.tensor(x["inf"]) * (x["mask"] - 1)[:, None, None]]
+    if share:
+        x["bias"] = torch.zeros(b // share, shape[3], shape[1], nk, dtype=dtype)
+    compare(x, *rounded_reference(x, terms), share)
