@@ -513,7 +513,7 @@ def cross_attention_supported(module, s, k_in, bias, mask=None):
             and s.dtype == k_in.dtype == torch.float32 and s.is_cuda and k_in.is_cuda
             and s.shape[0] == k_in.shape[0] and s.shape[-1] == k_in.shape[-1] == module.c_s
             and bias.dim() == 4 and tuple(bias.shape[1:]) == (heads, s.shape[1], k_in.shape[1])
-            and bias.shape[0] >= 1 and s.shape[0] % bias.shape[0] == 0 and bias.device == s.device
+            and (s.shape[0] % bias.shape[0] if bias.shape[0] else s.shape[0]) == 0 and bias.device == s.device
             and (mask is None or tuple(mask.shape) == tuple(k_in.shape[:2]))
             and all(p.bias is None for p in (module.proj_k, module.proj_v, module.proj_g)))
 

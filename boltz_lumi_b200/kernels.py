@@ -624,14 +624,14 @@ def _attention_args(q, k, v, bias, mask, inf, gate, scale):
         gate = _attention_rows(gate, dtype, "gate", (b, nq, h, d))
         gate_ptr, gate_stride = gate.data_ptr(), gate.stride()
     if bias is not None:
-        if bias.dtype != dtype or bias.dim() != 4 or tuple(bias.shape[1:]) != (h, nq, nk) or bias.shape[0] < 1 \
-                or b % bias.shape[0]:
+        if bias.dtype != dtype or bias.dim() != 4 or tuple(bias.shape[1:]) != (h, nq, nk) \
+                or (b % bias.shape[0] if bias.shape[0] else b):
             raise RuntimeError(f"bias must be {dtype} [B', {h}, {nq}, {nk}] with B' dividing {b}, got {bias.dtype} "
                                f"{list(bias.shape)}")
         if bias.stride(3) != 1 and nk > 1:
             planes = padded_planes(*bias.shape, device, dtype)
             bias = planes.copy_(bias)
-        bias_ptr, bias_stride, share = bias.data_ptr(), bias.stride(), b // bias.shape[0]
+        bias_ptr, bias_stride, share = bias.data_ptr(), bias.stride(), b // bias.shape[0] if b else 1
     if mask is not None:
         if tuple(mask.shape) != (b, nk):
             raise RuntimeError(f"mask must be [{b}, {nk}], got {list(mask.shape)}")
@@ -724,6 +724,8 @@ def cross_attention_backward(grad, q, k, v, out, lse, bias=None, mask=None, inf=
     dbias, ld = None, 0
     if bias is not None and need_bias_grad:
         dbias = padded_planes(*bias.shape, device, dtype)
+        if b == 0:
+            dbias.zero_()  # a bias that no sample reads
         ld = (x.nk + 7) // 8 * 8
     nbytes = size_of("bl_cross_attention_workspace", x)
     work = _workspace(nbytes, device)
