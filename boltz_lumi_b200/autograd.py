@@ -4,6 +4,8 @@
 :mod:`boltz_lumi_b200.kernels` with autograd recorded: ``loss.backward()`` runs the library's backward kernels.  Without
 grad mode or inputs that need a gradient they are the plain calls.
 
+They have reverse-mode gradients of first order: an input that carries a forward-mode tangent is refused.
+
 Under CUDA graph capture they refuse inputs that need a gradient.  A captured autograd pass would run the leaves' gradient
 accumulation on whatever stream an earlier, still living eager graph of the same leaves recorded, which ends the process
 inside torch; capture the explicit pair instead (``kernels.cross_attention(..., return_lse=True)`` and
@@ -17,6 +19,7 @@ from . import kernels
 
 def _recorded(name, *tensors):
     """Whether the call records autograd; refuses to do so under stream capture."""
+    kernels._refuse_tangents(*tensors)
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
         return False
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():

@@ -526,6 +526,7 @@ def cross_attend_with_bias(self, s, bias, mask, k_in, residual=None):
         raise RuntimeError(f"cross attention covers fp32 CUDA s [B, Nq, H*d] and k_in [B, Nk, H*d] with d % 8 == 0, "
                            f"d <= 128, bias [B', H, Nq, Nk] and mask [B, Nk]; got s {tuple(s.shape)}, "
                            f"k_in {tuple(k_in.shape)}, bias {tuple(bias.shape)}")
+    kernels._require_inference(s, bias, k_in, residual)
     heads, d = self.num_heads, self.head_dim
     with torch.autocast("cuda", enabled=False):  # the reference's math is fp32 throughout
         qg = _linear32(self, "_bl_w3_qg", s, [self.proj_q.weight, self.proj_g.weight], [self.proj_q.bias, None])

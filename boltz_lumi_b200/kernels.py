@@ -12,9 +12,17 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, launch, ptr, size_of, stream_of
+
+
+def _refuse_tangents(*tensors):
+    if forward_ad._current_level >= 0:  # inside dual_level(): the kernels would drop a tangent
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("boltz_lumi_b200 operators have no forward-mode derivatives (an input carries a tangent)")
 
 
 def _require_inference(*tensors):
@@ -22,6 +30,7 @@ def _require_inference(*tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("boltz_lumi_b200 kernels are inference-only (grad mode with requires_grad inputs)")
+    _refuse_tangents(*tensors)
 
 
 def _require_cuda(*tensors):
