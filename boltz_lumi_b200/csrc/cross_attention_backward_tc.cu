@@ -250,8 +250,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           for (int e = 0; e < 4; ++e)
             y[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
         }
-        __syncwarp();
-        if (half == 1 && lane == 0) tc::mbar_arrive(b_empty + bs);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
@@ -297,6 +295,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       // dQ has read the dS of tile j - 2 in this buffer.
       if (half == 0 && j >= 2 && !(ok = warp_wait(k_empty + (j - 2) % KS, ((j - 2) / KS) & 1, p.status, 0x40E))) break;
       tc::tmem_st_32x32b_x16(lanes + kDsCol + set * 32 + 16 * half, ds);
+      // The bias block is free once its values have gone into dS.  Released right after its loads, the next block
+      // overtook them where the stores of dbias held them up.
+      if (kBias && half == 1) {
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(b_empty + bs);
+      }
       if (kBias && dbias) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -590,6 +595,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       if (!ok) break;
       tc::tmem_st_wait();
       tc::tc_fence_before();
+      if (kBias) tc::fence_proxy_async_smem();  // the bias block has been read
       __syncwarp();
       if (lane == 0) {
         tc::mbar_arrive(stat_empty + s);
@@ -803,8 +809,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[e] = first ? z[e] : add2(acc[e], z[e]);
       if ((u + 1) % a.share == 0) {
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(b_empty + (jt & 1));
         if (i < a.nq) {
           Bf *dst = static_cast<Bf *>(p.x.dbias) + ((int64_t(bb) * a.heads + h) * a.nq + i) * p.x.dbias_ld;
 #pragma unroll
@@ -821,6 +825,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 if (k + e < a.nk) reinterpret_cast<uint16_t *>(dst)[k + e] = uint16_t(w[e >> 1] >> (16 * (e & 1)));
           }
         }
+        tc::fence_proxy_async_smem();  // the bias block has been read
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(b_empty + (jt & 1));
       }
     }
   }

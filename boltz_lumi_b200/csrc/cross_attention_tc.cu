@@ -311,8 +311,6 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
                         pack2(w[e] << 16, w[e] & 0xffff0000u));
           }
         }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(b_empty + t * BS + bs);
       } else {
 #pragma unroll
         for (int p = 0; p < 32; ++p)
@@ -373,7 +371,13 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
       // P of tile j - 2 was in this buffer.  Its P.V has read it: it was issued before S of
       // this tile, whose commit (s_full) covers every earlier product of that thread.
       const uint32_t p_col = lanes + S::kPCol + buf * 32;
-      if (__any_sync(0xffffffffu, far_row(m))) {
+      const bool far = __any_sync(0xffffffffu, far_row(m));  // every score has been looked at: the bias is in registers
+      if constexpr (kBias) {
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(b_empty + t * BS + bs);
+      }
+      if (far) {
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {

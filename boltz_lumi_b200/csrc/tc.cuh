@@ -109,7 +109,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsign
 // Proxy fences
 // ---------------------------------------------------------------------------
 // Generic-proxy writes to shared memory become visible to the async proxy
-// (tcgen05.mma operand reads, TMA stores).
+// (tcgen05.mma operand reads, TMA stores), and generic-proxy reads are over
+// before a TMA load overwrites what they read: an mbarrier arrival alone does
+// not wait for loads of the warp that are still in flight.
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
