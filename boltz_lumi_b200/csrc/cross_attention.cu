@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(32 * Step<T, DP>::warps) step_kernel(const Arg
   if (split > 1) cluster_barrier();  // peers may still be reading this CTA's parts
 }
 
-// Clusters of s CTAs that the device holds at once (1 / s of its SMs where the query fails).
+// Clusters of s CTAs that the device holds at once (1 / s of its SMs where the query fails; asked of the first device in
+// use: only the choice of a split hangs on it).
 template <typename T, int DP> int active_clusters(int s) {
   using S = Step<T, DP>;
   static const std::array<int, 9> table = [] {
@@ -544,8 +545,8 @@ template <typename T, int DP> int launch_step(const Args &a, cudaStream_t stream
   static_assert(S::bytes <= 232448, "shared memory");
   const int64_t slabs = int64_t(a.batch) * (a.heads / a.group);
   BL_CUDA(ensure_smem_limit(reinterpret_cast<const void *>(step_kernel<T, DP>), S::bytes));
-  // The split with the fewest waves per CTA's share of the keys, at least one chunk per warp.  (A fixed split of
-  // eight took two waves at 20 slabs: 62 us against 31.)
+  // The split with the fewest waves per CTA's share of the keys, at least one chunk per warp.  (At 20 slabs a fixed split
+  // of eight takes two waves: it took 62 us where six took 31, which later steps brought to 25.)
   int split = 1;
   double best = 0.;
   for (int e = 1; e <= 8 && (e == 1 || a.nk >= int64_t(e) * S::warps * S::kc); ++e) {

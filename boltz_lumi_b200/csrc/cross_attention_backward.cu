@@ -16,11 +16,14 @@
 //                  dbias where no other sample shares the bias;
 //   bias_kernel    one CTA = one block of a shared bias: dbias summed over its samples;
 //   window_kernel  all four gradients of small fp32 windows at once.
-// bf16 over 64 queries goes to cross_attention_backward_tc.cu (measured there).  What bounds these
-// kernels is the issue of the warp products: in fp32 each is three (tf32 pairs), and a CTA's
+// bf16 goes to cross_attention_backward_tc.cu (measured there) where back_covered says so: 64 keys or more,
+// more than 64 queries (or what worth_tiles allows), operands that tensor maps describe, bias rows
+// on 16-byte boundaries; a shared bias' gradient also wants d <= 64 (bias_tc).  The rest stays here.  What
+// bounds these kernels is the issue of the warp products: in fp32 each is three (tf32 pairs), and a CTA's
 // 16-row products read and split every operand tile again (10 x 8 x 96 x 6619 x 48, fp32, one bias
-// per five samples: 2.1 ms, 11 TFLOP/s of the formula's products; the plain form's library products
-// take about as long there and at d = 128).  Half the tile (16 rows) at d = 128, for two CTAs per SM, was
+// per five samples: 2.1 ms, 11 TFLOP/s of the formula's products, where the plain form's library products take
+// 1.85 ms; 22 x 16 x 33 x 752 x 128: 3 % slower than they).  A shared bias' gradient at d = 128, bf16, 2 x 16 x 384 x
+// 1734: 148 us here beside 128 us for the other gradients on tiles (at d = 64 37 beside 108).  Half the tile (16 rows) at d = 128, for two CTAs per SM, was
 // faster with few queries (961 -> 783 us) and slower else (1715 -> 1960 us).
 #include "cross_attention_backward.cuh"
 

@@ -16,6 +16,8 @@
 // tiles, a thread per resident row (TMEM lane), in two halves of 32 scores.  S and dP have two
 // buffers, so one set's products run under the other's arithmetic.  There is no row maximum to
 // agree on: the forward's statistics give p directly.  A gated do enters dP and dV as two bf16 terms.
+// P^T and dS^T (dS in the query kernel) are rounded to bf16 once, as the operands of their products; an unshared
+// bias' gradient is that dS.  A shared one adds dS in fp32 and rounds the sum.
 //
 // Against the same loops on warp products: 4 x 16(4) x 777 x 2048 x 128 without bias, dk/dv 446 ->
 // 138 us, dq 435 -> 133 us (five products, 620 TFLOP/s); 2 x 16 x 384 x 1734 x 48 with a shared bias and a

@@ -10,7 +10,9 @@
 //   * the thread adds the bias row from shared memory (128-byte swizzle: conflict-free
 //     16-byte reads), takes p = exp2 and writes P as bf16 to one of two TMEM buffers;
 //   * O += P V with P from TMEM and V in its natural [key][d] order (MN-major);
-//     O is rescaled only when a row's maximum grew by more than 2^8.
+//     O is rescaled only when a row's maximum grew by more than 2^8 (a published refinement of the
+//     online softmax: any reference near the maximum serves, as P and the row sum share it).
+// P is rounded to bf16 for its product; the row sum adds the fp32 values.
 // 2 x 16 x 2048 x 8190 x 48 with one bias: 385 us (floor 92 us: 606 MB, nearly all the bias); 4 x 16(4) x
 // 777 x 2048 x 128 without: 112 us, 465 TFLOP/s.  What bounds it: the softmax warps' chain per tile, two
 // warps per scheduler deep (1430 cycles per 128 x 64 scores, of which the exponentials, 16 per clock and
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(Shape<kTiles, kBlocks, kBias>::kThreads, kTile
   }
 }
 
-// Clusters of s CTAs that the device holds at once.
+// Clusters of s CTAs that the device holds at once (asked of the first device in use: only the choice of a split hangs on it).
 template <int kTiles, int kBlocks, bool kBias> int active_clusters(int s) {
   using S = Shape<kTiles, kBlocks, kBias>;
   static const std::array<int, 9> table = [] {
@@ -538,7 +540,7 @@ int launch_tc(const Args &a, const CUtensorMap (&maps)[4], cudaStream_t stream) 
   x.split = 1;
   if (kTiles == 1) {
     // Few CTAs: a cluster divides the keys, by the waves that it takes (128 queries, 8 heads: 33 -> 12 us at
-    // 1024 keys, 164 -> 29 us at 8192; 2 x 16 x 384 x 1734: 46 -> 39 us).
+    // 1024 keys, 164 -> 29 us at 8192; 2 x 16 x 384 x 1734 without a mask: 46 -> 39 us).
     const int64_t work = (a.nk + kBK - 1) / kBK;
     double best = 0.;
     for (int e = 1; e <= 8 && (e == 1 || e <= work); ++e) {
@@ -579,7 +581,8 @@ int forward_tc(const Args &a, cudaStream_t stream, bool *taken) {
   }
   *taken = true;
   const bool wide = a.d > 64;
-  // Two query tiles per CTA once they still give every SM a CTA.
+  // Two query tiles per CTA once they still give every SM a CTA.  (Up to 128 queries the second tile has no rows: one tile
+  // per CTA and two CTAs per SM would take 66 against 95 us at 1024 heads x 128 x 512 x 32, 140 against 122 us at d = 128.)
   const bool two = int64_t((a.nq + 2 * kBQ - 1) / (2 * kBQ)) * a.heads * a.batch >= num_sms();
   if (a.bias) {
     if (two) return wide ? launch_tc<2, 2, true>(a, maps, stream) : launch_tc<2, 1, true>(a, maps, stream);

@@ -99,9 +99,13 @@ constexpr float kFar = 1024.f;
 __device__ __forceinline__ bool far_row(float m) { return fabsf(m) > kFar && fabsf(m) != INFINITY; }
 
 __device__ __forceinline__ int n_words(int nk) { return (nk + 31) / 32; }
-// At most 64 queries leave half or more of a tile's rows idle: worth it over many keys while the heads do not fill
-// the GPU.  32 queries to 4096 keys, forward and gradients in us, against the kernels on warp products: 8 heads 19 / 89
-// against 144 / 201, 64 heads 49 / 182 against 148 / 267, 512 heads 299 / 985 against 133 / 520; equal at 128 keys.
+// At most 64 queries leave half or more of a tile's rows idle: taken over many keys while the heads do not fill the
+// GPU.  Forward and gradients of 32 queries in us (d = 64, no bias, no mask), against the kernels on warp products, which
+// divide the keys among clusters too: 8 heads, 256 keys 13 / 24 against 16 / 26, 4096 keys 22 / 79 against 25 / 46; 64 heads,
+// 256 keys 17 / 26 against 16 / 28, 4096 keys 49 / 169 against 41 / 124; 148 heads, 1024 keys 28 / 87 against 29 / 79; past
+// the limit, 192 heads, 256 keys 28 / 48 against 17 / 40, 512 heads, 1024 keys 83 / 286 against 49 / 200.  At 128 keys
+// (every head count) the warp products are as fast or faster.  The rule follows the forward of few heads; gradients over
+// 1024 keys or more and the forward of 64 heads are slower by it.
 inline bool worth_tiles(const Args &a) {
   return a.nq > 64 || (a.nk >= 256 && int64_t(a.heads) * a.batch <= num_sms());
 }

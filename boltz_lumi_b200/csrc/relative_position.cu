@@ -14,8 +14,9 @@
 // Both forwards are bound by their HBM writes and both gradients by reading
 // the upstream gradient once.  Encoding of 512 tokens, 128 fp32 channels: 31 us for 134 MB (4.3 TB/s; a plain
 // fill of the same tensor 21 us; the table's load and the launch are the rest).  Its gradient at 424 tokens: 40 us
-// for 92 MB, of which the partial sums' kernel is 4 us; six private tables of 36 KB leave six warps per SM, whose
-// instructions are the limit.  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
+// for 92 MB, of which the partial sums' kernel is 4 us; six private tables of 36 KB leave six warps per SM, 1.5 per
+// scheduler, whose latency is the limit: they issue in 25 % of the cycles, and of 6.0 cycles per issue 1.7 wait for an
+// instruction's own latency, 1.5 for loads and 0.6 for shared memory (DRAM at 30 %).  Bias planes of 16 x 2048 x 8190 in bf16: 97 us for 537 MB (5.5 TB/s; a plain fill 74 to 90 us).
 // Table gradient of 2 x 16 x 768 x 1134 fp32: 47 us for 112 MB, 12 us of it clearing and adding up the histograms.  The gradients are deterministic: every partial
 // sum belongs to one thread, and partials are added in a fixed order.
 #include <type_traits>
@@ -609,7 +610,10 @@ int bias_check(const char *name, const BiasArgs &a) {
 }
 
 int bias_lut_bytes(int distance) { return (2 * distance + 1) * 2; }
-int bias_grad_heads(int buckets) { return buckets <= 48 ? 4 : 1; }  // 2 KB (4 heads) or 0.5 KB (1) per bucket
+// 2 KB (4 heads) or 0.5 KB (1) of histogram per bucket.  Four heads share the index work of a row while two CTAs fit an SM:
+// 2 x 16 x 768 x 1134 fp32, cold, 33 buckets 58 us with four heads and 120 with one, 48 buckets 93 and 120, 65 to 92 buckets (one
+// CTA per SM) 128 and 120.
+int bias_grad_heads(int buckets) { return buckets <= 48 ? 4 : 1; }
 // Launch shape of the table gradient: up to three CTAs per SM (67 KB of histogram at 33 buckets x 4 heads), each with
 // one column block and one run of rows, in whole groups of four rows.
 struct BiasGrad {

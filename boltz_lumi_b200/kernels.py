@@ -681,6 +681,9 @@ def cross_attention(q, k, v, bias=None, mask=None, inf=None, gate=None, scale=No
     AttentionPairBias).  ``scale`` defaults to d ** -0.5.  A query whose keys are all left out gets zeros.
 
     Scores, softmax statistics and sums are fp32; bf16 probabilities are rounded to bf16 for the product with ``v``.
+    ``q`` and the keys and values that a bool mask does not leave out are finite: fp32 products split them into two
+    terms, so an infinity (or a magnitude of 2^127 and more) may give NaN where the formula has an infinity.  ``bias``
+    may hold -inf.
     Returns [B, Nq, H, d], with ``return_lse`` also the :class:`AttentionStats` that :func:`cross_attention_backward`
     takes (``rows.sum(0)`` is the log-sum-exp of the scores).
     """
@@ -705,7 +708,7 @@ def cross_attention_backward(grad, q, k, v, out, lse, bias=None, mask=None, inf=
 
     ``grad`` is the gradient of ``out``; the other arguments are the forward call's, ``out`` and ``lse`` (an
     :class:`AttentionStats`) its results.
-    ``dk`` and ``dv`` are summed over the query heads that share a key/value head and ``dbias`` ([B', H, Nq, Nk], rows on
+    In bf16 p and ds are rounded to bf16 for their products.  ``dk`` and ``dv`` are summed over the query heads that share a key/value head and ``dbias`` ([B', H, Nq, Nk], rows on
     16-byte boundaries) over the samples that share a bias, in fp32 and in a fixed order: the same inputs give the same
     bits.  The mask is a constant.  ``need_bias_grad=False`` skips dbias.
     """

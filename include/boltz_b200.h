@@ -471,6 +471,8 @@ BL_API int bl_relative_position_bias_backward(const void *grad, int dtype, int64
  * mask_kind 0: none; 1: uint8 [batch][nk], keys with 0 are left out, whatever
  * their k, v and bias hold; 2: fp32 [batch][nk], x += inf * (mask - 1).
  * A query whose keys are all left out (mask, -inf bias or nk = 0) gets 0.
+ * Other q, k, v and dy are finite (fp32: below 2^127 in magnitude, as products split
+ * them into two terms); an infinity there may come out as NaN.
  * gate may be NULL; out: [batch][nq][heads][head_dim] contiguous; lse (NULL:
  * not wanted): fp32 [2][batch][heads][nq], a reference of the row's scores (their
  * maximum or a little below it; -inf for a query without keys) and the log of the
