@@ -222,100 +222,100 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           cut = bits[2 * j + half];
         } else {
           cut = __ballot_sync(0xffffffffu, mask_value(a, b, k0 + lane) != 0.f);
-      }
-      const bool adds = cut && a.mask_kind == kMaskAdd;
-      if (adds) {
-        const float v = mask_value(a, b, k0 + lane);
-        __syncwarp();
-        mk[lane] = v == -INFINITY ? 0.f : v;
-        cut = __ballot_sync(0xffffffffu, v == -INFINITY);  // from here on: keys that count nothing
-        __syncwarp();
-      }
-      if (half == 0) {
-        if (!(ok = warp_wait(s_full + set, (j >> 1) & 1, p.status, 0x407))) break;
-        tc::tc_fence_after();
-        if constexpr (kBias) ok = warp_wait(b_full + bs, (j / BS) & 1, p.status, 0x408);
-        if (!ok) break;
-      }
-      uint32_t sv[32], dv[32];
-      tc::tmem_ld_32x32b_x32(lanes + set * kPair + kSCol + 32 * half, sv);
-      tc::tmem_ld_32x32b_x32(lanes + set * kPair + kDpCol + 32 * half, dv);
-      tc::tmem_ld_wait_regs(sv, dv);
-      uint64_t y[16];
-      if constexpr (kBias) {
-        const uint32_t brow = smem_addr(smem + S::kBiasOff + bs * S::kB) + row * 128;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 v = lds128(brow + (((4 * half + c) ^ (row & 7)) << 4));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            y[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
         }
-      } else {
+        const bool adds = cut && a.mask_kind == kMaskAdd;
+        if (adds) {
+          const float v = mask_value(a, b, k0 + lane);
+          __syncwarp();
+          mk[lane] = v == -INFINITY ? 0.f : v;
+          cut = __ballot_sync(0xffffffffu, v == -INFINITY);  // from here on: keys that count nothing
+          __syncwarp();
+        }
+        if (half == 0) {
+          if (!(ok = warp_wait(s_full + set, (j >> 1) & 1, p.status, 0x407))) break;
+          tc::tc_fence_after();
+          if constexpr (kBias) ok = warp_wait(b_full + bs, (j / BS) & 1, p.status, 0x408);
+          if (!ok) break;
+        }
+        uint32_t sv[32], dv[32];
+        tc::tmem_ld_32x32b_x32(lanes + set * kPair + kSCol + 32 * half, sv);
+        tc::tmem_ld_32x32b_x32(lanes + set * kPair + kDpCol + 32 * half, dv);
+        tc::tmem_ld_wait_regs(sv, dv);
+        uint64_t y[16];
+        if constexpr (kBias) {
+          const uint32_t brow = smem_addr(smem + S::kBiasOff + bs * S::kB) + row * 128;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
-      }
-      if (adds)
+          for (int c = 0; c < 4; ++c) {
+            const uint4 v = lds128(brow + (((4 * half + c) ^ (row & 7)) << 4));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = add2(y[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
-      uint32_t ds[16];
-      if (far)
+            for (int e = 0; e < 4; ++e)
+              y[4 * c + e] = fma2(pack2(sv[8 * c + 2 * e], sv[8 * c + 2 * e + 1]), scale2, pack2(w[e] << 16, w[e] & 0xffff0000u));
+          }
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          y[e] = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
-      else
+          for (int e = 0; e < 16; ++e) y[e] = mul2(pack2(sv[2 * e], sv[2 * e + 1]), scale2);
+        }
+        if (adds)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = fma2(y[e], log2e2, c2);
+          for (int e = 0; e < 16; ++e) y[e] = add2(y[e], *reinterpret_cast<const uint64_t *>(mk + 2 * e));
+        uint32_t ds[16];
+        if (far)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint64_t prob = pack2(__float_as_uint(fast_exp2(lo_f(y[e]))), __float_as_uint(fast_exp2(hi_f(y[e]))));
-        const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
-        ds[e] = pack_bf16x2(lo_f(g), hi_f(g));
-      }
-      if (cut) {
+          for (int e = 0; e < 16; ++e)
+            y[e] = pack2(__float_as_uint(fmaf(lo_f(y[e]) - m, kLog2e, nl)), __float_as_uint(fmaf(hi_f(y[e]) - m, kLog2e, nl)));
+        else
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] = fma2(y[e], log2e2, c2);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const uint32_t c = cut >> (2 * e);
-          ds[e] &= (c & 1 ? 0u : 0xffffu) | (c & 2 ? 0u : 0xffff0000u);
+          const uint64_t prob = pack2(__float_as_uint(fast_exp2(lo_f(y[e]))), __float_as_uint(fast_exp2(hi_f(y[e]))));
+          const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), delta2));
+          ds[e] = pack_bf16x2(lo_f(g), hi_f(g));
         }
-        // K rows of left-out keys must be zero before dS meets them in dQ.
-        if (a.mask_kind == kMaskKeep) {
-          const int ks = j % KS, key = 8 * quarter + (lane >> 2);
-          if (cut >> key & 1) {
-            wait_phase(k_full + ks, (j / KS) & 1, p.status, 0x409);  // complete: S came from this stage
-            uint8_t *k = smem + S::kKOff + ks * S::kStr + (32 * half + key) * 128 + (lane & 3) * 32;
+        if (cut) {
 #pragma unroll
-            for (int c = 0; c < kBlocks; ++c)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<uint4 *>(k + c * kTileTc * 128 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t c = cut >> (2 * e);
+            ds[e] &= (c & 1 ? 0u : 0xffffu) | (c & 2 ? 0u : 0xffff0000u);
           }
+          // K rows of left-out keys must be zero before dS meets them in dQ.
+          if (a.mask_kind == kMaskKeep) {
+            const int ks = j % KS, key = 8 * quarter + (lane >> 2);
+            if (cut >> key & 1) {
+              wait_phase(k_full + ks, (j / KS) & 1, p.status, 0x409);  // complete: S came from this stage
+              uint8_t *k = smem + S::kKOff + ks * S::kStr + (32 * half + key) * 128 + (lane & 3) * 32;
+#pragma unroll
+              for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  *reinterpret_cast<uint4 *>(k + c * kTileTc * 128 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            tc::fence_proxy_async_smem();
+          }
+        }
+        // dQ has read the dS of tile j - 2 in this buffer.
+        if (half == 0 && j >= 2 && !(ok = warp_wait(k_empty + (j - 2) % KS, ((j - 2) / KS) & 1, p.status, 0x40E))) break;
+        tc::tmem_st_32x32b_x16(lanes + kDsCol + set * 32 + 16 * half, ds);
+        // The bias block is free once its values have gone into dS.  Released right after its loads, the next block
+        // overtook them where the stores of dbias held them up.
+        if (kBias && half == 1) {
           tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(b_empty + bs);
         }
-      }
-      // dQ has read the dS of tile j - 2 in this buffer.
-      if (half == 0 && j >= 2 && !(ok = warp_wait(k_empty + (j - 2) % KS, ((j - 2) / KS) & 1, p.status, 0x40E))) break;
-      tc::tmem_st_32x32b_x16(lanes + kDsCol + set * 32 + 16 * half, ds);
-      // The bias block is free once its values have gone into dS.  Released right after its loads, the next block
-      // overtook them where the stores of dbias held them up.
-      if (kBias && half == 1) {
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(b_empty + bs);
-      }
-      if (kBias && dbias) {
+        if (kBias && dbias) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int k = k0 + 8 * c;
-          if (k + 8 <= a.nk)
-            *reinterpret_cast<uint4 *>(dbias + k) = make_uint4(ds[4 * c], ds[4 * c + 1], ds[4 * c + 2], ds[4 * c + 3]);
-          else
+          for (int c = 0; c < 4; ++c) {
+            const int k = k0 + 8 * c;
+            if (k + 8 <= a.nk)
+              *reinterpret_cast<uint4 *>(dbias + k) = make_uint4(ds[4 * c], ds[4 * c + 1], ds[4 * c + 2], ds[4 * c + 3]);
+            else
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (k + e < a.nk) reinterpret_cast<uint16_t *>(dbias)[k + e] = uint16_t(ds[4 * c + (e >> 1)] >> (16 * (e & 1)));
+              for (int e = 0; e < 8; ++e)
+                if (k + e < a.nk) reinterpret_cast<uint16_t *>(dbias)[k + e] = uint16_t(ds[4 * c + (e >> 1)] >> (16 * (e & 1)));
+          }
         }
-      }
       }
       if (!ok) break;
       tc::tmem_st_wait();
@@ -570,29 +570,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           } else {
             z[e] = fma2(pack2(sv[2 * e], sv[2 * e + 1]), scale2, mk2);
           }
-      }
-      if (far)
+        }
+        if (far)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
-                       __float_as_uint(fmaf(hi_f(z[e]) - st[2 * e + 1], kLog2e, st[kTileTc + 2 * e + 1])));
-      else
+          for (int e = 0; e < 16; ++e)
+            z[e] = pack2(__float_as_uint(fmaf(lo_f(z[e]) - st[2 * e], kLog2e, st[kTileTc + 2 * e])),
+                         __float_as_uint(fmaf(hi_f(z[e]) - st[2 * e + 1], kLog2e, st[kTileTc + 2 * e + 1])));
+        else
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = fma2(z[e], log2e2, *reinterpret_cast<const uint64_t *>(st + 2 * kTileTc + 2 * e));
+          for (int e = 0; e < 16; ++e) z[e] = fma2(z[e], log2e2, *reinterpret_cast<const uint64_t *>(st + 2 * kTileTc + 2 * e));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p0 = fast_exp2(lo_f(z[e])), p1 = fast_exp2(hi_f(z[e]));
-        const uint64_t prob = pack2(__float_as_uint(p0), __float_as_uint(p1));
-        const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), *reinterpret_cast<const uint64_t *>(st + 3 * kTileTc + 2 * e)));
-        pt[e] = out ? 0u : pack_bf16x2(p0, p1);
-        ds[e] = out ? 0u : pack_bf16x2(lo_f(g), hi_f(g));
-      }
-      // Wide rows: over columns that this half or the first one has read.  Else dV and dK have
-      // read what tile u - 2 left here.
-      if (kBlocks == 1 && half == 0 && u >= 2 && !(ok = warp_wait(st_empty + (u - 2) % ST, ((u - 2) / ST) & 1, p.status, 0x420)))
-        break;
-      tc::tmem_st_32x32b_x16(lanes + C::pt + set * C::pt_step + 16 * half, pt);
-      tc::tmem_st_32x32b_x16(lanes + C::ds + set * C::pt_step + 16 * half, ds);
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = fast_exp2(lo_f(z[e])), p1 = fast_exp2(hi_f(z[e]));
+          const uint64_t prob = pack2(__float_as_uint(p0), __float_as_uint(p1));
+          const uint64_t g = mul2(prob, add2(pack2(dv[2 * e], dv[2 * e + 1]), *reinterpret_cast<const uint64_t *>(st + 3 * kTileTc + 2 * e)));
+          pt[e] = out ? 0u : pack_bf16x2(p0, p1);
+          ds[e] = out ? 0u : pack_bf16x2(lo_f(g), hi_f(g));
+        }
+        // Wide rows: over columns that this half or the first one has read.  Else dV and dK have
+        // read what tile u - 2 left here.
+        if (kBlocks == 1 && half == 0 && u >= 2 && !(ok = warp_wait(st_empty + (u - 2) % ST, ((u - 2) / ST) & 1, p.status, 0x420)))
+          break;
+        tc::tmem_st_32x32b_x16(lanes + C::pt + set * C::pt_step + 16 * half, pt);
+        tc::tmem_st_32x32b_x16(lanes + C::ds + set * C::pt_step + 16 * half, ds);
       }
       if (!ok) break;
       tc::tmem_st_wait();
